@@ -295,6 +295,124 @@ int rsm_fcollect(size_t elem_size, uint64_t team, void *dest, const void *source
  * (context_ib_device_coll.cpp:105-120). */
 int rsm_barrier_all(int iterations, const rsm_launch_t *launch);
 
+/* ---- row collectives: the operators of a model spread over PEs -------------------------------
+ * No counterpart in the reference.  Each member of a team holds a part of a model; these calls
+ * close the work that the members did apart, on whole rows (tokens) of a batch, in one pass over
+ * the data.  They belong between the calls that make their operands on the same stream and need no
+ * barrier of their own: stream order is the barrier, the launch makes every member's results, and
+ * other PEs' slices are not touched.  They only launch kernels, so they can be recorded in a graph.
+ *
+ * Operands are symmetric arrays (addresses in PE 0's slice) of RSM_FLOAT or RSM_BF16 elements, as
+ * `dtype` says; sums and everything between are 32-bit floats, every result is rounded once, and
+ * every run gives the same bits.  Row strides (*_ld) are in elements, 0 = packed rows; rows may
+ * start at any element.  A call checks its operands as the other entry points do, refuses results
+ * that overlap other operands (one array for both is allowed where it says so), and writes nothing
+ * beyond the rows and columns it names. */
+
+enum rsm_norm_flags {
+  RSM_NORM_POST = 1,        /* the members' sum goes through a norm of its own               */
+  RSM_NORM_REPLICATED = 2   /* every member holds the whole residual stream                  */
+};
+
+/* The end of a block and the norm in front of the next.  With s = the members' sum of a row of
+ * `source`, r(v) = 1 / sqrt(mean(v^2) + eps) and o = weight_offset:
+ *   z            = s r(s) (o + post_weight)  with RSM_NORM_POST (without post_weight: s r(s)); s otherwise
+ *   residual_out = residual_scale * residual + block_scale * gate * z      (without gate: 1)
+ *   normed       = residual_out r(residual_out) (o + pre_weight)           (without pre_weight: 1)
+ * `normed` goes to every member.  Row i of the residual stream is read and written on its owner, the
+ * member i / share with share = ceil(rows / team size), at row i % share of arrays of `share` rows; with
+ * RSM_NORM_REPLICATED the arrays have all rows on every member, the owner's copy is read and every
+ * member's is written.  `total` (may be NULL) keeps s for the backward pass: share rows, packed, on the
+ * owners.  The weights (cols elements) and `gate` (one packed row for every rows_per_gate rows of the
+ * batch; 0 = one row for all) hold the same values on every member.  `normed` may be NULL, may be
+ * `source` (equal strides), and residual_out may be `residual`.  cols <= 16384, rows < 2^22, eps > 0. */
+typedef struct rsm_norm_args {
+  int dtype;
+  int flags;                 /* rsm_norm_flags */
+  uint64_t team;
+  size_t rows, cols, rows_per_gate;
+  float eps, residual_scale, block_scale, weight_offset;
+  size_t source_ld, residual_ld, normed_ld;   /* residual_ld: residual and residual_out */
+  const void *source, *residual, *pre_weight, *post_weight, *gate;
+  void *residual_out, *normed, *total;
+} rsm_norm_args_t;
+int rsm_norm_to_all(const rsm_norm_args_t *args, void *stream);
+
+/* Its gradient.  `grad_normed` holds every member's part of the gradient of the next block's input
+ * (its rows are summed over the members; NULL: none), grad_residual_out the gradient that comes down
+ * the residual stream (held as the stream is; NULL: none), residual_out and total what the forward pass
+ * left (total: needed with RSM_NORM_POST and for grad_gate).  Results: grad_source, the gradient of every
+ * member's part, the same on all of them; grad_residual (may be NULL), held as the stream is; and,
+ * where they are not NULL, 32-bit sums over the rows on every member: grad_pre_weight and
+ * grad_post_weight (cols floats), grad_gate (gate's shape).  grad_source may be grad_normed (equal
+ * strides) and grad_residual may be grad_residual_out.  `work`: rsm_norm_grad_work_bytes() bytes of a
+ * symmetric array that no other call in flight uses (the first member's copy is written); not needed
+ * when none of the sums is asked for.  normed_ld: grad_normed's, source_ld: grad_source's,
+ * residual_ld: the stream's arrays'. */
+typedef struct rsm_norm_grad_args {
+  int dtype;
+  int flags;
+  uint64_t team;
+  size_t rows, cols, rows_per_gate;
+  float eps, residual_scale, block_scale, weight_offset;
+  size_t source_ld, residual_ld, normed_ld;
+  const void *grad_normed, *grad_residual_out, *residual_out, *total, *pre_weight, *post_weight, *gate;
+  void *grad_source, *grad_residual;
+  float *grad_pre_weight, *grad_post_weight, *grad_gate;
+  void *work;
+} rsm_norm_grad_args_t;
+int rsm_norm_to_all_grad(const rsm_norm_grad_args_t *args, void *stream);
+/* Bytes of `work` for these sizes, flags and gate. */
+int rsm_norm_grad_work_bytes(const rsm_norm_grad_args_t *args, size_t *bytes);
+
+/* Log probabilities over a vocabulary split over the team: member m holds the logits of ids
+ * m * shard .. min(vocab, (m + 1) * shard) - 1 (shard 0: ceil(vocab / team size)), one row per token
+ * position.  With y = scale * logits over all members:
+ *   lse = ln sum exp(y), logprob = y[token] - lse, entropy = -sum p ln p with p = exp(y - lse),
+ * and the top_k largest logits (at most 32), equal ones by ascending id, with their log probabilities.
+ * Results go to every member; those that are NULL are left out.  `tokens` (the first member's copy is
+ * read) are ids; a negative one stands for a position without a token: logprob 0.  An id of vocab or
+ * more gives NaN and raises the status word (rsm_take_status() == 2).  Logits at minus infinity are
+ * outside the vocabulary; a row of nothing else has lse and log probabilities of minus infinity and
+ * entropy 0.  A row with a NaN or plus infinity has NaN results; NaN logits are never alternatives, and
+ * where fewer than top_k others are there the rest of the row is id -1 with NaN.
+ * `work` (rsm_logprob_work_bytes() bytes) and pSync (ROC_SHMEM_REDUCE_SYNC_SIZE longs, all
+ * ROC_SHMEM_SYNC_VALUE on entry and on return) are symmetric arrays that no other call in flight uses;
+ * the first member's copies serve batches of fewer than 256 rows, and larger ones need neither (0
+ * bytes).  rows < 2^22, vocab < 2^30, scale > 0. */
+typedef struct rsm_logprob_args {
+  int dtype;
+  int top_k;
+  uint64_t team;
+  size_t rows, vocab, shard, logits_ld;
+  float scale;
+  const void *logits;
+  const int64_t *tokens;
+  float *logprob, *entropy, *lse;     /* [rows] */
+  int32_t *top_ids;                   /* [rows][top_k] */
+  float *top_logprobs;                /* [rows][top_k] */
+  void *work;
+  long *pSync;
+} rsm_logprob_args_t;
+int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream);
+int rsm_logprob_work_bytes(const rsm_logprob_args_t *args, size_t *bytes);
+
+/* Its gradient: every member's part of the gradient of the logits, from the gradients of logprob,
+ * entropy and lse (NULL: none; positions without a token have none of logprob) and what the forward
+ * pass gave as lse and entropy (needed for grad_entropy).  The first member's copies of the arrays of
+ * [rows] are read.  grad_logits may be `logits` (equal strides). */
+typedef struct rsm_logprob_grad_args {
+  int dtype;
+  uint64_t team;
+  size_t rows, vocab, shard, logits_ld, grad_ld;
+  float scale;
+  const void *logits;
+  const int64_t *tokens;
+  const float *lse, *entropy, *grad_logprob, *grad_entropy, *grad_lse;
+  void *grad_logits;
+} rsm_logprob_grad_args_t;
+int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream);
+
 /* ---- small puts and AMOs ------------------------------------------------------
  * Thread t of the grid issues ops[t], ops[t+T], ... (T = total threads) through
  * the thread-level API (roc_shmem.hpp:907-1147; context_ib_device.cpp:84-184,

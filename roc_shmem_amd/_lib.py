@@ -13,6 +13,56 @@ class Launch(C.Structure):
 
 LP = C.POINTER(Launch)
 
+
+class RowArgs(C.Structure):
+    """Arguments of a row collective by name; operands are symmetric arrays or addresses.  A field
+    that is not given has the value of `_defaults_`, or 0 / NULL."""
+    _defaults_ = {}
+
+    def __init__(self, **fields):
+        super().__init__()
+        for name, value in {**self._defaults_, **fields}.items():
+            if name not in self._names_:
+                raise TypeError("%s has no field %r" % (type(self).__name__, name))
+            setattr(self, name, value)
+
+    def __setattr__(self, name, value):
+        if name not in self._names_:
+            raise AttributeError("%s has no field %r" % (type(self).__name__, name))
+        super().__setattr__(name, getattr(value, "addr", value))
+
+
+def _row_args(name, doc, fields, **defaults):
+    return type(name, (RowArgs,), {"__doc__": doc, "_fields_": fields, "_names_": frozenset(f for f, _ in fields),
+                                   "_defaults_": defaults})
+
+
+def _pointers(names):
+    return [(n, vp) for n in names.split()]
+
+
+_NORM_NUMBERS = ([("dtype", i32), ("flags", i32), ("team", u64), ("rows", sz), ("cols", sz), ("rows_per_gate", sz)] +
+                 [(n, C.c_float) for n in ("eps", "residual_scale", "block_scale", "weight_offset")] +
+                 [("source_ld", sz), ("residual_ld", sz), ("normed_ld", sz)])
+NormArgs = _row_args(
+    "NormArgs", "rsm_norm_args_t", _NORM_NUMBERS +
+    _pointers("source residual pre_weight post_weight gate residual_out normed total"),
+    eps=1e-6, residual_scale=1.0, block_scale=1.0)
+NormGradArgs = _row_args(
+    "NormGradArgs", "rsm_norm_grad_args_t", _NORM_NUMBERS +
+    _pointers("grad_normed grad_residual_out residual_out total pre_weight post_weight gate grad_source "
+              "grad_residual grad_pre_weight grad_post_weight grad_gate work"),
+    eps=1e-6, residual_scale=1.0, block_scale=1.0)
+LogprobArgs = _row_args(
+    "LogprobArgs", "rsm_logprob_args_t",
+    [("dtype", i32), ("top_k", i32), ("team", u64), ("rows", sz), ("vocab", sz), ("shard", sz), ("logits_ld", sz),
+     ("scale", C.c_float)] + _pointers("logits tokens logprob entropy lse top_ids top_logprobs work pSync"), scale=1.0)
+LogprobGradArgs = _row_args(
+    "LogprobGradArgs", "rsm_logprob_grad_args_t",
+    [("dtype", i32), ("team", u64), ("rows", sz), ("vocab", sz), ("shard", sz), ("logits_ld", sz), ("grad_ld", sz),
+     ("scale", C.c_float)] +
+    _pointers("logits tokens lse entropy grad_logprob grad_entropy grad_lse grad_logits"), scale=1.0)
+
 # name -> (restype, argtypes); every symbol declared in include/rocshmem_mi355x.h
 SIGNATURES = {
     "rsm_init": (i32, [i32, sz, i32, C.c_uint]),
@@ -66,6 +116,12 @@ SIGNATURES = {
     "rsm_alltoall": (i32, [sz, u64, vp, vp, sz, LP]),
     "rsm_fcollect": (i32, [sz, u64, vp, vp, sz, LP]),
     "rsm_barrier_all": (i32, [i32, LP]),
+    "rsm_norm_to_all": (i32, [C.POINTER(NormArgs), vp]),
+    "rsm_norm_to_all_grad": (i32, [C.POINTER(NormGradArgs), vp]),
+    "rsm_norm_grad_work_bytes": (i32, [C.POINTER(NormGradArgs), C.POINTER(sz)]),
+    "rsm_logprob_to_all": (i32, [C.POINTER(LogprobArgs), vp]),
+    "rsm_logprob_to_all_grad": (i32, [C.POINTER(LogprobGradArgs), vp]),
+    "rsm_logprob_work_bytes": (i32, [C.POINTER(LogprobArgs), C.POINTER(sz)]),
     "rsm_small_ops": (i32, [vp, sz, vp, LP]),
     "rsm_sq_flush_target": (i32, [i32, C.POINTER(C.c_uint64), C.POINTER(C.c_uint32)]),
     "rsm_sq_reset": (i32, []),

@@ -20,6 +20,9 @@ __all__ = [
     "roc_shmem_rma",
     "roc_shmem_broadcast", "roc_shmem_team_broadcast", "roc_shmem_alltoall",
     "roc_shmem_fcollect", "roc_shmem_wg_barrier_all", "roc_shmem_small_ops",
+    "roc_shmem_norm_to_all", "roc_shmem_norm_to_all_grad", "roc_shmem_norm_grad_work_bytes",
+    "roc_shmem_logprob_to_all", "roc_shmem_logprob_to_all_grad", "roc_shmem_logprob_work_bytes",
+    "NormArgs", "NormGradArgs", "LogprobArgs", "LogprobGradArgs", "NORM_POST", "NORM_REPLICATED",
     "sq_reset", "sq_read", "sq_image", "sq_state", "sq_constants", "sq_rkey", "sq_flush_target",
     "sq_consume", "sq_set_mode", "sq_consumer_state", "sq_consumer_start", "sq_consumer_stop",
     "sq_consumer_running", "cq_reader_state", "cq_image", "atomic_ret_image", "arena",
@@ -43,6 +46,7 @@ THREAD, WAVE, WG, WG_SHARED = range(4)
 (OP_P64, OP_FADD64, OP_ADD64, OP_FINC64, OP_INC64, OP_CSWAP64, OP_FETCH64, OP_SET64, OP_SWAP64,
  OP_P32, OP_FADD32, OP_PUTMEM, OP_GETMEM, OP_FAND64, OP_FOR64, OP_FXOR64) = range(16)
 OP_NONE = 255
+NORM_POST, NORM_REPLICATED = 1, 2
 ROC_SHMEM_REDUCE_SYNC_SIZE = 256
 ROC_SHMEM_BCAST_SYNC_SIZE = 256
 
@@ -386,6 +390,56 @@ def roc_shmem_small_ops(ops_dev, n_ops, fetched_dev=None, launch=None):
     _check(L.load().rsm_small_ops(_addr(ops_dev), n_ops,
                                   _addr(fetched_dev) if fetched_dev is not None else None,
                                   _launch(launch)))
+
+
+# ---- row collectives: the operators of a model spread over PEs -----------------------------
+#
+# The arguments are a structure that a program fills once and passes again and again; it must
+# outlive no call, since a call reads it before it returns.
+
+from ._lib import LogprobArgs, LogprobGradArgs, NormArgs, NormGradArgs  # noqa: E402
+
+
+def _row_call(name, args, stream):
+    _check(getattr(L.load(), name)(args, getattr(stream, "h", stream)))
+
+
+def _row_bytes(name, args):
+    n = C.c_size_t(0)
+    _check(getattr(L.load(), name)(args, C.byref(n)))
+    return n.value
+
+
+def roc_shmem_norm_to_all(args, stream=None):
+    """The end of a block: the members' parts summed, normalised, gated and scaled into the residual
+    stream, and the next block's normalised input on every member (rsm_norm_to_all; NormArgs)."""
+    _row_call("rsm_norm_to_all", args, stream)
+
+
+def roc_shmem_norm_to_all_grad(args, stream=None):
+    """Gradient of roc_shmem_norm_to_all (rsm_norm_to_all_grad; NormGradArgs)."""
+    _row_call("rsm_norm_to_all_grad", args, stream)
+
+
+def roc_shmem_norm_grad_work_bytes(args):
+    """Bytes of NormGradArgs.work for these sizes, flags and gate."""
+    return _row_bytes("rsm_norm_grad_work_bytes", args)
+
+
+def roc_shmem_logprob_to_all(args, stream=None):
+    """Log probabilities of given tokens, entropies, normalisers and the likeliest alternatives over a
+    vocabulary split over the team (rsm_logprob_to_all; LogprobArgs)."""
+    _row_call("rsm_logprob_to_all", args, stream)
+
+
+def roc_shmem_logprob_to_all_grad(args, stream=None):
+    """Gradient of roc_shmem_logprob_to_all (rsm_logprob_to_all_grad; LogprobGradArgs)."""
+    _row_call("rsm_logprob_to_all_grad", args, stream)
+
+
+def roc_shmem_logprob_work_bytes(args):
+    """Bytes of LogprobArgs.work for these sizes."""
+    return _row_bytes("rsm_logprob_work_bytes", args)
 
 
 # ---- send queues and wave-level drivers -----------------------------------------------------

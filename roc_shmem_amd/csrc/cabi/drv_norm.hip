@@ -1,0 +1,670 @@
+// C ABI: the end of a block whose partial outputs lie on the members of a team, and its gradient
+// (rsm_norm_to_all, rsm_norm_to_all_grad; no counterpart in the reference).
+//
+// With s the members' sum of a row, C its length, r(v) = 1 / sqrt(mean(v^2) + eps) and o the weight
+// offset:
+//   z  = s r(s) (o + w_post)   (RSM_NORM_POST; z = s otherwise)
+//   x' = a x + b g z           x the residual stream, a and b its and the block's scale, g the gate
+//   h  = x' r(x') (o + w_pre)  the next block's input, on every member
+// and backwards, with dh the members' sum of the gradients of h and n = x' r(x'), u = s r(s):
+//   t  = dh (o + w_pre)        D = dx' + r(x') (t - n mean(t n))      dw_pre = sum_rows dh n
+//   dx = a D                   f = b D g       dg = sum_rows b D z    dw_post = sum_rows f u
+//   ds = r(s) (q - u mean(q u)), q = f (o + w_post)   (RSM_NORM_POST; ds = f otherwise)
+//
+// Sums, means and everything between a load and a store are 32-bit floats; every output is rounded
+// to its type once.  Members are summed in ascending order, so every run gives the same bits.
+#include <cmath>
+
+#include "roc_shmem.hpp"
+#include "rocshmem_device/rows.hpp"
+#include "rows_common.hpp"
+
+using namespace rocshmem;
+using namespace rocshmem::detail;
+
+namespace {
+
+constexpr int kMaxCols = 16384;
+
+// What both kernels know of a call.  Pointers are the first member's copies, `step` bytes lead to
+// the next member's; row strides are in elements.
+struct NormShape {
+  int rows, cols, members, share;   // row i is held by member i / share (its owner)
+  int rows_per_gate;
+  int64_t step;
+  int64_t partial_ld, residual_ld, normed_ld;
+  float eps, inv_cols, residual_scale, block_scale, weight_offset;
+  bool post, replicated;
+};
+
+struct NormForward {
+  NormShape s;
+  const char *source, *residual, *pre_weight, *post_weight, *gate;
+  char *residual_out, *normed, *total;
+};
+
+struct NormBackward {
+  NormShape s;
+  const char *grad_normed, *residual_out, *total, *grad_residual_out, *pre_weight, *post_weight, *gate;
+  char *grad_source, *grad_residual, *grad_gate;
+  float *part_pre, *part_post, *part_gate;   // [units][part_ld], null where nobody asks for them
+  int part_ld;
+  // A unit (the lanes that hold a row) walks the rows of its own.  `direct`: whole gate groups,
+  // rows_per_unit of them a multiple of rows_per_gate; otherwise units_per_gate units share a group.
+  int units, units_per_gate, rows_per_unit;
+  bool direct;
+};
+
+template <typename T>
+__device__ __forceinline__ const T *row_at(const char *base, int64_t bytes, int64_t row, int64_t ld, int col) {
+  return reinterpret_cast<const T *>(base + bytes) + row * ld + col;
+}
+template <typename T>
+__device__ __forceinline__ T *row_at(char *base, int64_t bytes, int64_t row, int64_t ld, int col) {
+  return reinterpret_cast<T *>(base + bytes) + row * ld + col;
+}
+
+constexpr int kFoldDepth = 8;   // members whose loads are in flight together
+
+// Sum over the members of one row's elements that this lane holds.
+template <typename T, int kLanes, int NV, bool kTail>
+__device__ __forceinline__ void fold_members(const NormShape &s, const char *base, int64_t row, int64_t ld,
+                                             int lane, float (&acc)[NV][kRowVec<T>]) {
+  constexpr int V = kRowVec<T>;
+  constexpr int kDepth = NV >= 4 ? 2 : NV == 2 ? 4 : kFoldDepth;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[v][e] = 0.f;
+  for (int m = 0; m < s.members; m += kDepth) {
+    u32x4 raw[kDepth][NV];
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * kLanes + lane) * V;
+        raw[k][v] = u32x4{0u, 0u, 0u, 0u};
+        if (m + k < s.members) raw[k][v] = row_load<T, kTail>(row_at<T>(base, (m + k) * s.step, row, ld, c), s.cols - c);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k)
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[v][e] += row_get<T>(raw[k][v], e);
+  }
+}
+
+template <typename T, int kLanes, int NV, bool kTail>
+__device__ __forceinline__ void load_row(const T *p, int cols, int lane, u32x4 (&raw)[NV]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * kLanes + lane) * kRowVec<T>;
+    raw[v] = row_load<T, kTail>(p + c, cols - c);
+  }
+}
+
+// The row to `copies` members, `step` bytes apart.
+template <typename T, int kLanes, int NV, bool kTail>
+__device__ __forceinline__ void store_row(T *p, int64_t step, int copies, int cols, int lane,
+                                          const float (&f)[NV][kRowVec<T>]) {
+  u32x4 raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) raw[v] = row_pack<T>(f[v]);
+  for (int m = 0; m < copies; ++m) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * kLanes + lane) * kRowVec<T>;
+      row_store<T, kTail>(bytes_on(p, m * step) + c, cols - c, raw[v]);
+    }
+  }
+}
+
+template <int kLanes>
+constexpr int kWgLanes = kLanes < 256 ? 256 : kLanes;
+
+template <typename T, int kLanes, int NV, bool kTail>
+__global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
+  constexpr int V = kRowVec<T>;
+  __shared__ float slots[2 * (kWgLanes<kLanes> / 64)];
+  int turn = 0;
+  const NormShape &s = p.s;
+  const int lane = threadIdx.x % kLanes;
+  const int row = uniform(static_cast<int>(blockIdx.x * (kWgLanes<kLanes> / kLanes) + threadIdx.x / kLanes));
+  if (row >= s.rows) return;   // a whole wave of a workgroup of one-wave rows; no barrier follows
+  const int owner = uniform(row / s.share);
+  const int64_t home = owner * s.step;
+  const int64_t held = s.replicated ? row : row - owner * s.share;
+
+  u32x4 x[NV], wpre[NV], wpost[NV], gate[NV];
+  load_row<T, kLanes, NV, kTail>(row_at<T>(p.residual, home, held, s.residual_ld, 0), s.cols, lane, x);
+  if (p.pre_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, wpre);
+  if (p.post_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.post_weight, home, 0, 0, 0), s.cols, lane, wpost);
+  if (p.gate)
+    load_row<T, kLanes, NV, kTail>(row_at<T>(p.gate, home, row / s.rows_per_gate, s.cols, 0), s.cols, lane, gate);
+
+  float acc[NV][V];
+  fold_members<T, kLanes, NV, kTail>(s, p.source, row, s.partial_ld, lane, acc);
+  if (p.total) store_row<T, kLanes, NV, kTail>(row_at<T>(p.total, home, row - owner * s.share, s.cols, 0), 0, 1, s.cols, lane, acc);
+
+  if (s.post) {
+    float ss[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss[0] = fmaf(acc[v][e], acc[v][e], ss[0]);
+    row_sums<kLanes>(ss, slots, turn);
+    const float r = rsqrtf(fmaf(ss[0], s.inv_cols, s.eps));
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float w = p.post_weight ? s.weight_offset + row_get<T>(wpost[v], e) : 1.f;
+        acc[v][e] *= r * w;
+      }
+  }
+  float ss[1] = {0.f};
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float z = acc[v][e];
+      if (p.gate) z *= row_get<T>(gate[v], e);
+      acc[v][e] = fmaf(s.residual_scale, row_get<T>(x[v], e), s.block_scale * z);
+      ss[0] = fmaf(acc[v][e], acc[v][e], ss[0]);
+    }
+  store_row<T, kLanes, NV, kTail>(row_at<T>(p.residual_out, s.replicated ? 0 : home, held, s.residual_ld, 0), s.step,
+                                  s.replicated ? s.members : 1, s.cols, lane, acc);
+  if (!p.normed) return;
+  row_sums<kLanes>(ss, slots, turn);
+  const float r = rsqrtf(fmaf(ss[0], s.inv_cols, s.eps));
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float w = p.pre_weight ? s.weight_offset + row_get<T>(wpre[v], e) : 1.f;
+      acc[v][e] *= r * w;
+    }
+  store_row<T, kLanes, NV, kTail>(row_at<T>(p.normed, 0, row, s.normed_ld, 0), s.step, s.members, s.cols, lane, acc);
+}
+
+// A lane's sums over the rows of its unit, as 32-bit floats to row `at` of an array.
+template <typename T, int kLanes, int NV>
+__device__ __forceinline__ void store_part(float *part, int64_t at, int ld, int cols, int lane, const float (&f)[NV][kRowVec<T>]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * kLanes + lane) * kRowVec<T>;
+#pragma unroll
+    for (int k = 0; k < kRowVec<T>; k += 4) {
+      // part_ld is a multiple of 4, so a group of four that begins inside the row stays inside it
+      if (c + k < cols)
+        *reinterpret_cast<float4 *>(part + at * ld + c + k) = float4{f[v][k], f[v][k + 1], f[v][k + 2], f[v][k + 3]};
+    }
+  }
+}
+
+template <typename T, int kLanes, int NV, bool kTail>
+__global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackward p) {
+  constexpr int V = kRowVec<T>;
+  __shared__ float slots[2 * 3 * (kWgLanes<kLanes> / 64)];
+  __shared__ float slots1[2 * (kWgLanes<kLanes> / 64)];
+  int turn = 0, turn1 = 0;
+  const NormShape &s = p.s;
+  const int lane = threadIdx.x % kLanes;
+  const int unit = uniform(static_cast<int>(blockIdx.x * (kWgLanes<kLanes> / kLanes) + threadIdx.x / kLanes));
+  if (unit >= p.units) return;   // as in norm_kernel
+  int64_t first, last;
+  if (p.direct) {
+    first = static_cast<int64_t>(unit) * p.rows_per_unit;
+    last = first + p.rows_per_unit;
+  } else {
+    const int64_t group = unit / p.units_per_gate, end = (group + 1) * s.rows_per_gate;
+    first = group * s.rows_per_gate + static_cast<int64_t>(unit % p.units_per_gate) * p.rows_per_unit;
+    last = first + p.rows_per_unit < end ? first + p.rows_per_unit : end;
+  }
+  if (last > s.rows) last = s.rows;
+
+  float sum_pre[NV][V], sum_post[NV][V], sum_gate[NV][V];
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum_pre[v][e] = sum_post[v][e] = sum_gate[v][e] = 0.f;
+
+  for (int64_t row = first; row < last; ++row) {
+    const int owner = uniform(static_cast<int>(row) / s.share);
+    const int64_t home = owner * s.step, shared = row - static_cast<int64_t>(owner) * s.share;
+    const int64_t held = s.replicated ? row : shared;
+    const int gate_row = uniform(static_cast<int>(row) / s.rows_per_gate);
+    u32x4 x[NV], tot[NV], din[NV], w[NV];
+    load_row<T, kLanes, NV, kTail>(row_at<T>(p.residual_out, home, held, s.residual_ld, 0), s.cols, lane, x);
+    if (p.total) load_row<T, kLanes, NV, kTail>(row_at<T>(p.total, home, shared, s.cols, 0), s.cols, lane, tot);
+    if (p.grad_residual_out)
+      load_row<T, kLanes, NV, kTail>(row_at<T>(p.grad_residual_out, home, held, s.residual_ld, 0), s.cols, lane, din);
+    float d[NV][V];
+    if (p.grad_normed) {
+      fold_members<T, kLanes, NV, kTail>(s, p.grad_normed, row, s.normed_ld, lane, d);
+      if (p.pre_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, w);
+    }
+    // sum x'^2, sum t x' and sum s^2 in one go: the second mean is r(x') times a plain sum
+    float sums[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (p.grad_normed) {
+          const float xe = row_get<T>(x[v], e);
+          const float t = d[v][e] * (p.pre_weight ? s.weight_offset + row_get<T>(w[v], e) : 1.f);
+          sums[0] = fmaf(xe, xe, sums[0]);
+          sums[1] = fmaf(t, xe, sums[1]);
+        }
+        if (s.post) sums[2] = fmaf(row_get<T>(tot[v], e), row_get<T>(tot[v], e), sums[2]);
+      }
+    row_sums<kLanes>(sums, slots, turn);
+    const float r2 = rsqrtf(fmaf(sums[0], s.inv_cols, s.eps));
+    const float mean_tn = sums[1] * r2 * s.inv_cols;
+    const float r1 = rsqrtf(fmaf(sums[2], s.inv_cols, s.eps));
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float dd = p.grad_residual_out ? row_get<T>(din[v], e) : 0.f;
+        if (p.grad_normed) {
+          const float n = row_get<T>(x[v], e) * r2;
+          const float t = d[v][e] * (p.pre_weight ? s.weight_offset + row_get<T>(w[v], e) : 1.f);
+          sum_pre[v][e] = fmaf(d[v][e], n, sum_pre[v][e]);
+          dd = fmaf(r2, fmaf(-n, mean_tn, t), dd);
+        }
+        d[v][e] = dd;
+      }
+    if (p.grad_residual) {
+      float dx[NV][V];
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < V; ++e) dx[v][e] = s.residual_scale * d[v][e];
+      store_row<T, kLanes, NV, kTail>(row_at<T>(p.grad_residual, s.replicated ? 0 : home, held, s.residual_ld, 0), s.step,
+                                      s.replicated ? s.members : 1, s.cols, lane, dx);
+    }
+    // from here on d is f, and then q
+    u32x4 g[NV];
+    if (p.gate) load_row<T, kLanes, NV, kTail>(row_at<T>(p.gate, home, gate_row, s.cols, 0), s.cols, lane, g);
+    if (p.post_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.post_weight, home, 0, 0, 0), s.cols, lane, w);
+    float qs[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float f = s.block_scale * d[v][e];
+        const float wp = p.post_weight ? s.weight_offset + row_get<T>(w[v], e) : 1.f;
+        const float u = p.total ? row_get<T>(tot[v], e) * (s.post ? r1 : 1.f) : 0.f;
+        if (p.gate) {
+          sum_gate[v][e] = fmaf(f, s.post ? u * wp : u, sum_gate[v][e]);
+          f *= row_get<T>(g[v], e);
+        }
+        if (s.post) {
+          sum_post[v][e] = fmaf(f, u, sum_post[v][e]);
+          f *= wp;
+          qs[0] = fmaf(f, u, qs[0]);
+        }
+        d[v][e] = f;
+      }
+    if (s.post) {
+      row_sums<kLanes>(qs, slots1, turn1);
+      const float mean_qu = qs[0] * s.inv_cols;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[v][e] = r1 * fmaf(-mean_qu * r1, row_get<T>(tot[v], e), d[v][e]);
+    }
+    store_row<T, kLanes, NV, kTail>(row_at<T>(p.grad_source, 0, row, s.partial_ld, 0), s.step, s.members, s.cols, lane, d);
+    if (p.direct && p.grad_gate && (row + 1 == last || (row + 1) % s.rows_per_gate == 0)) {
+      for (int m = 0; m < s.members; ++m) {
+        float *out = reinterpret_cast<float *>(p.grad_gate + m * s.step) + static_cast<int64_t>(gate_row) * s.cols;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const int c = (v * kLanes + lane) * V + e;
+            if (c < s.cols) out[c] = sum_gate[v][e];
+          }
+      }
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum_gate[v][e] = 0.f;
+    }
+  }
+  if (p.part_pre) store_part<T, kLanes, NV>(p.part_pre, unit, p.part_ld, s.cols, lane, sum_pre);
+  if (p.part_post) store_part<T, kLanes, NV>(p.part_post, unit, p.part_ld, s.cols, lane, sum_post);
+  if (p.part_gate) store_part<T, kLanes, NV>(p.part_gate, unit, p.part_ld, s.cols, lane, sum_gate);
+}
+
+// The units' sums, added up in ascending order of a fixed tree: workgroup (x, y) makes columns
+// 64 x .. 64 x + 63 of sum y (0: pre_weight, 1: post_weight, then the gate rows) and writes them to
+// every member.
+struct PartSums {
+  const float *part_pre, *part_post, *part_gate;
+  char *grad_pre, *grad_post, *grad_gate;
+  int units, units_per_gate, part_ld, cols, members;
+  int64_t step;
+};
+
+__global__ void __launch_bounds__(256) part_sums_kernel(PartSums p) {
+  __shared__ float4 sums[16][17];
+  const int y = blockIdx.y;
+  const float *part = y == 0 ? p.part_pre : y == 1 ? p.part_post : p.part_gate;
+  char *out = y == 0 ? p.grad_pre : y == 1 ? p.grad_post : p.grad_gate;
+  if (!out) return;
+  const int quad = threadIdx.x % 16, rank = threadIdx.x / 16;
+  const int c = (blockIdx.x * 16 + quad) * 4;
+  int first = 0, count = p.units;
+  if (y >= 2) {
+    first = (y - 2) * p.units_per_gate;
+    count = p.units_per_gate;
+  }
+  float4 sum{0.f, 0.f, 0.f, 0.f};
+  if (c < p.cols) {
+#pragma unroll 8
+    for (int u = rank; u < count; u += 16) {
+      const float4 a = *reinterpret_cast<const float4 *>(part + static_cast<int64_t>(first + u) * p.part_ld + c);
+      sum.x += a.x;
+      sum.y += a.y;
+      sum.z += a.z;
+      sum.w += a.w;
+    }
+  }
+  sums[rank][quad] = sum;
+  __syncthreads();
+  if (rank != 0 || c >= p.cols) return;
+  for (int k = 1; k < 16; ++k) {
+    const float4 a = sums[k][quad];
+    sum.x += a.x;
+    sum.y += a.y;
+    sum.z += a.z;
+    sum.w += a.w;
+  }
+  const float each[4] = {sum.x, sum.y, sum.z, sum.w};
+  for (int m = 0; m < p.members; ++m) {
+    float *to = reinterpret_cast<float *>(out + m * p.step) + (y >= 2 ? static_cast<int64_t>(y - 2) * p.cols : 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < p.cols) to[c + e] = each[e];
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------
+
+// Lanes per row and vectors per lane: the fewest of either that hold the row.
+struct RowLanes {
+  int lanes, vecs;
+};
+RowLanes lanes_for(int cols, int vec) {
+  static const RowLanes choices[] = {{64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 1}, {512, 2}, {1024, 1}, {1024, 2}, {1024, 4}};
+  for (const RowLanes &c : choices)
+    if (c.lanes * c.vecs * vec >= cols) return c;
+  return {0, 0};
+}
+
+template <typename T, int kLanes, int NV, typename P>
+void launch_rows(const P &p, int units, bool tail, hipStream_t stream) {
+  const unsigned per_wg = kWgLanes<kLanes> / kLanes;
+  const dim3 grid((static_cast<unsigned>(units) + per_wg - 1) / per_wg), block(kWgLanes<kLanes>);
+  if constexpr (std::is_same<P, NormForward>::value) {
+    if (tail) hipLaunchKernelGGL((norm_kernel<T, kLanes, NV, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((norm_kernel<T, kLanes, NV, false>), grid, block, 0, stream, p);
+  } else {
+    if (tail) hipLaunchKernelGGL((norm_grad_kernel<T, kLanes, NV, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((norm_grad_kernel<T, kLanes, NV, false>), grid, block, 0, stream, p);
+  }
+}
+
+template <typename T, typename P>
+void launch_for(const P &p, int units, RowLanes l, hipStream_t stream) {
+  const bool tail = p.s.cols % kRowVec<T> != 0;
+  switch (l.lanes * 8 + l.vecs) {
+    case 64 * 8 + 1: launch_rows<T, 64, 1>(p, units, tail, stream); break;
+    case 64 * 8 + 2: launch_rows<T, 64, 2>(p, units, tail, stream); break;
+    case 256 * 8 + 1: launch_rows<T, 256, 1>(p, units, tail, stream); break;
+    case 256 * 8 + 2: launch_rows<T, 256, 2>(p, units, tail, stream); break;
+    case 512 * 8 + 1: launch_rows<T, 512, 1>(p, units, tail, stream); break;
+    case 512 * 8 + 2: launch_rows<T, 512, 2>(p, units, tail, stream); break;
+    case 1024 * 8 + 1: launch_rows<T, 1024, 1>(p, units, tail, stream); break;
+    case 1024 * 8 + 2: launch_rows<T, 1024, 2>(p, units, tail, stream); break;
+    default:
+      if constexpr (sizeof(T) == 4) launch_rows<T, 1024, 4>(p, units, tail, stream);
+  }
+}
+
+template <typename P>
+void launch_typed(int dtype, const P &p, int units, RowLanes l, hipStream_t stream) {
+  if (dtype == RSM_BF16) launch_for<__hip_bfloat16>(p, units, l, stream);
+  else launch_for<float>(p, units, l, stream);
+}
+
+size_t type_size(int dtype) { return dtype == RSM_FLOAT ? 4 : dtype == RSM_BF16 ? 2 : 0; }
+
+// What a call's sizes and numbers come to, or false with the error set.  A = either argument struct.
+template <typename A>
+bool shape_of(const A &a, const char *call, size_t partial_ld, size_t normed_ld, rsm::Members *members, NormShape *out) {
+  const std::string who = std::string(call) + ": ";
+  auto refuse = [&](const char *why) {
+    rsm::fail(who + why);
+    return false;
+  };
+  if (!type_size(a.dtype)) return refuse("dtype must be RSM_FLOAT or RSM_BF16");
+  if (a.flags & ~(RSM_NORM_POST | RSM_NORM_REPLICATED)) return refuse("unknown flags");
+  if (a.cols < 1 || a.cols > kMaxCols) return refuse("cols must be in [1, 16384]");
+  if (a.rows >= 1u << 22) return refuse("rows must be below 2^22");
+  if (partial_ld < a.cols || normed_ld < a.cols || (a.residual_ld && a.residual_ld < a.cols))
+    return refuse("a row stride is shorter than a row");
+  const size_t far = ~size_t{0} >> 24;
+  if (partial_ld > far / (a.rows + 1) || normed_ld > far / (a.rows + 1) || a.residual_ld > far / (a.rows + 1))
+    return refuse("a row stride is too long");
+  if (!(a.eps > 0.f) || !std::isfinite(a.eps)) return refuse("eps must be a positive number");
+  if (!std::isfinite(a.residual_scale) || !std::isfinite(a.block_scale) || !std::isfinite(a.weight_offset))
+    return refuse("scales and the weight offset must be finite");
+  if (a.post_weight && !(a.flags & RSM_NORM_POST)) return refuse("post_weight without RSM_NORM_POST");
+  if (!rsm::members_of(a.team, call, members)) return false;
+  const rsm::Members &team = *members;
+  NormShape s{};
+  s.rows = static_cast<int>(a.rows);
+  s.cols = static_cast<int>(a.cols);
+  s.members = team.size;
+  s.share = static_cast<int>((a.rows + team.size - 1) / team.size);
+  if (s.share < 1) s.share = 1;
+  s.rows_per_gate = a.rows_per_gate == 0 || a.rows_per_gate > a.rows ? (s.rows ? s.rows : 1) : static_cast<int>(a.rows_per_gate);
+  s.step = team.step;
+  s.partial_ld = static_cast<int64_t>(partial_ld);
+  s.normed_ld = static_cast<int64_t>(normed_ld);
+  s.residual_ld = static_cast<int64_t>(a.residual_ld ? a.residual_ld : a.cols);
+  s.eps = a.eps;
+  s.inv_cols = static_cast<float>(1.0 / static_cast<double>(a.cols));
+  s.residual_scale = a.residual_scale;
+  s.block_scale = a.block_scale;
+  s.weight_offset = a.weight_offset;
+  s.post = (a.flags & RSM_NORM_POST) != 0;
+  s.replicated = (a.flags & RSM_NORM_REPLICATED) != 0;
+  *out = s;
+  return true;
+}
+
+size_t gate_rows(const NormShape &s) { return s.rows ? (static_cast<size_t>(s.rows) + s.rows_per_gate - 1) / s.rows_per_gate : 0; }
+
+// How the rows of a backward pass are dealt to units, and the room their sums take.
+struct GradPlan {
+  RowLanes lanes;
+  int units, units_per_gate, rows_per_unit, part_ld;
+  bool direct;
+  size_t part_bytes;   // of one of the arrays of sums
+  int parts;           // how many arrays there are
+};
+
+GradPlan plan_of(const NormShape &s, int dtype, bool has_gate) {
+  GradPlan g{};
+  g.lanes = lanes_for(s.cols, dtype == RSM_BF16 ? 8 : 4);
+  // enough units to fill the chip's 256 compute units, no more: each leaves its sums behind
+  const int64_t target = g.lanes.lanes == 64 ? 4096 : 256 * (1024 / g.lanes.lanes);
+  const int64_t per_unit = (s.rows + target - 1) / target;
+  const int64_t group = has_gate ? s.rows_per_gate : s.rows;
+  g.part_ld = (s.cols + 3) & ~3;
+  if (group <= per_unit && has_gate && gate_rows(s) > 1) {
+    g.direct = true;
+    g.rows_per_unit = static_cast<int>((per_unit + group - 1) / group * group);
+    g.units_per_gate = 0;
+    g.units = static_cast<int>((s.rows + g.rows_per_unit - 1) / g.rows_per_unit);
+  } else {
+    g.direct = false;
+    g.units_per_gate = static_cast<int>((group + per_unit - 1) / (per_unit ? per_unit : 1));
+    if (g.units_per_gate < 1) g.units_per_gate = 1;
+    g.rows_per_unit = static_cast<int>((group + g.units_per_gate - 1) / g.units_per_gate);
+    g.units = g.units_per_gate * static_cast<int>(has_gate ? gate_rows(s) : s.rows ? 1 : 0);
+  }
+  g.parts = 1 + (s.post ? 1 : 0) + (has_gate && !g.direct ? 1 : 0);
+  g.part_bytes = static_cast<size_t>(g.units) * g.part_ld * sizeof(float);
+  return g;
+}
+
+const char *moved(const void *p, int64_t bytes) { return p ? static_cast<const char *>(p) + bytes : nullptr; }
+char *moved(void *p, int64_t bytes) { return p ? static_cast<char *>(p) + bytes : nullptr; }
+
+}  // namespace
+
+extern "C" {
+
+int rsm_norm_to_all(const rsm_norm_args_t *args, void *stream) {
+  RSM_ENTRY;
+  const char *call = "norm_to_all";
+  if (!args) return rsm::fail("norm_to_all: arguments are NULL");
+  const rsm_norm_args_t &a = *args;
+  rsm::Members team;
+  NormShape s;
+  const size_t source_ld = a.source_ld ? a.source_ld : a.cols, normed_ld = a.normed_ld ? a.normed_ld : a.cols;
+  if (!a.source || !a.residual || !a.residual_out) return rsm::fail("norm_to_all: source, residual and residual_out must be given");
+  if (a.pre_weight && !a.normed) return rsm::fail("norm_to_all: pre_weight without normed");
+  if (!shape_of(a, call, source_ld, normed_ld, &team, &s)) return -1;
+  if (a.rows == 0) return 0;
+  const size_t size = type_size(a.dtype), held = s.replicated ? a.rows : s.share, ld = static_cast<size_t>(s.residual_ld);
+  rsm::Operands o(call);
+  o.matrix(a.source, "source", a.rows, a.cols, source_ld, size, false);
+  o.matrix(a.residual, "residual", held, a.cols, ld, size, false);
+  o.add(a.pre_weight, "pre_weight", a.cols * size, false);
+  o.add(a.post_weight, "post_weight", a.cols * size, false);
+  o.add(a.gate, "gate", gate_rows(s) * a.cols * size, false);
+  o.matrix(a.residual_out, "residual_out", held, a.cols, ld, size, true);
+  o.or_same_as(a.residual);
+  o.matrix(a.normed, "normed", a.rows, a.cols, normed_ld, size, true);
+  if (normed_ld == source_ld) o.or_same_as(a.source);
+  o.matrix(a.total, "total", s.share, a.cols, a.cols, size, true);
+  if (!o.ok()) return -1;
+  NormForward p{};
+  p.s = s;
+  p.source = moved(a.source, team.first);
+  p.residual = moved(a.residual, team.first);
+  p.pre_weight = moved(a.pre_weight, team.first);
+  p.post_weight = moved(a.post_weight, team.first);
+  p.gate = moved(a.gate, team.first);
+  p.residual_out = moved(a.residual_out, team.first);
+  p.normed = moved(a.normed, team.first);
+  p.total = moved(a.total, team.first);
+  launch_typed(a.dtype, p, s.rows, lanes_for(s.cols, a.dtype == RSM_BF16 ? 8 : 4), static_cast<hipStream_t>(stream));
+  return rsm::after_launch(call);
+}
+
+int rsm_norm_grad_work_bytes(const rsm_norm_grad_args_t *args, size_t *bytes) {
+  RSM_ENTRY;
+  const char *call = "norm_grad_work_bytes";
+  if (!args || !bytes) return rsm::fail("norm_grad_work_bytes: an argument is NULL");
+  rsm::Members team;
+  NormShape s;
+  if (!shape_of(*args, call, args->cols, args->cols, &team, &s)) return -1;
+  const GradPlan g = plan_of(s, args->dtype, args->gate != nullptr);
+  *bytes = g.part_bytes * g.parts;
+  return 0;
+}
+
+int rsm_norm_to_all_grad(const rsm_norm_grad_args_t *args, void *stream) {
+  RSM_ENTRY;
+  const char *call = "norm_to_all_grad";
+  if (!args) return rsm::fail("norm_to_all_grad: arguments are NULL");
+  const rsm_norm_grad_args_t &a = *args;
+  rsm::Members team;
+  NormShape s;
+  const size_t source_ld = a.source_ld ? a.source_ld : a.cols, normed_ld = a.normed_ld ? a.normed_ld : a.cols;
+  if (!a.grad_source) return rsm::fail("norm_to_all_grad: grad_source must be given");
+  if (!a.grad_normed && !a.grad_residual_out) return rsm::fail("norm_to_all_grad: neither grad_normed nor grad_residual_out is given");
+  if (a.grad_normed && !a.residual_out) return rsm::fail("norm_to_all_grad: grad_normed needs residual_out");
+  if (((a.flags & RSM_NORM_POST) || a.grad_gate) && !a.total) return rsm::fail("norm_to_all_grad: total must be given (with RSM_NORM_POST, or for grad_gate)");
+  if (a.grad_pre_weight && !a.grad_normed) return rsm::fail("norm_to_all_grad: grad_pre_weight without grad_normed");
+  if (a.grad_post_weight && !(a.flags & RSM_NORM_POST)) return rsm::fail("norm_to_all_grad: grad_post_weight without RSM_NORM_POST");
+  if (a.grad_gate && !a.gate) return rsm::fail("norm_to_all_grad: grad_gate without gate");
+  if (!shape_of(a, call, source_ld, normed_ld, &team, &s)) return -1;
+  const GradPlan g = plan_of(s, a.dtype, a.gate != nullptr);
+  const bool sums = a.grad_pre_weight || a.grad_post_weight || (a.grad_gate && !g.direct);
+  if (sums && s.rows && !a.work) return rsm::fail("norm_to_all_grad: work must be given (rsm_norm_grad_work_bytes)");
+  const size_t size = type_size(a.dtype), held = s.replicated ? a.rows : s.share, ld = static_cast<size_t>(s.residual_ld);
+  const size_t mine = a.rows ? held : 0, shared = a.rows ? s.share : 0;
+  rsm::Operands o(call);
+  o.matrix(a.grad_normed, "grad_normed", a.rows, a.cols, normed_ld, size, false);
+  o.matrix(a.residual_out, "residual_out", mine, a.cols, ld, size, false);
+  o.matrix(a.total, "total", shared, a.cols, a.cols, size, false);
+  o.matrix(a.grad_residual_out, "grad_residual_out", mine, a.cols, ld, size, false);
+  o.add(a.pre_weight, "pre_weight", a.cols * size, false);
+  o.add(a.post_weight, "post_weight", a.cols * size, false);
+  o.add(a.gate, "gate", gate_rows(s) * a.cols * size, false);
+  o.matrix(a.grad_source, "grad_source", a.rows, a.cols, source_ld, size, true);
+  if (source_ld == normed_ld) o.or_same_as(a.grad_normed);
+  o.matrix(a.grad_residual, "grad_residual", mine, a.cols, ld, size, true);
+  o.or_same_as(a.grad_residual_out);
+  o.add(a.grad_pre_weight, "grad_pre_weight", a.cols * 4, true);
+  o.add(a.grad_post_weight, "grad_post_weight", a.cols * 4, true);
+  o.add(a.grad_gate, "grad_gate", gate_rows(s) * a.cols * 4, true);
+  if (sums) o.add(a.work, "work (rsm_norm_grad_work_bytes)", g.part_bytes * g.parts, true);
+  if (!o.ok()) return -1;
+  if (!a.grad_gate && !sums && a.rows == 0) return 0;
+
+  NormBackward p{};
+  p.s = s;
+  p.grad_normed = moved(a.grad_normed, team.first);
+  p.residual_out = moved(a.residual_out ? a.residual_out : a.grad_residual_out, team.first);
+  p.total = moved(a.total, team.first);
+  p.grad_residual_out = moved(a.grad_residual_out, team.first);
+  p.pre_weight = moved(a.pre_weight, team.first);
+  p.post_weight = moved(a.post_weight, team.first);
+  p.gate = moved(a.gate, team.first);
+  p.grad_source = moved(a.grad_source, team.first);
+  p.grad_residual = moved(a.grad_residual, team.first);
+  p.grad_gate = moved(a.grad_gate, team.first);
+  float *part = reinterpret_cast<float *>(moved(a.work, team.first));
+  const size_t part_floats = g.part_bytes / sizeof(float);
+  if (a.grad_pre_weight) p.part_pre = part;
+  if (a.grad_post_weight) p.part_post = part + part_floats;
+  if (a.grad_gate && !g.direct) p.part_gate = part + part_floats * (s.post ? 2 : 1);
+  p.part_ld = g.part_ld;
+  p.units = g.units;
+  p.units_per_gate = g.units_per_gate;
+  p.rows_per_unit = g.rows_per_unit;
+  p.direct = g.direct;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (g.units) launch_typed(a.dtype, p, g.units, g.lanes, st);
+  if (sums) {
+    PartSums r{};
+    r.part_pre = p.part_pre;
+    r.part_post = p.part_post;
+    r.part_gate = p.part_gate;
+    r.grad_pre = moved(a.grad_pre_weight, team.first);
+    r.grad_post = moved(a.grad_post_weight, team.first);
+    r.grad_gate = p.part_gate ? p.grad_gate : nullptr;
+    r.units = g.units;
+    r.units_per_gate = g.units_per_gate;
+    r.part_ld = g.part_ld;
+    r.cols = s.cols;
+    r.members = s.members;
+    r.step = s.step;
+    const unsigned gates = p.part_gate ? static_cast<unsigned>(gate_rows(s)) : 0;
+    hipLaunchKernelGGL(part_sums_kernel, dim3((s.cols + 63) / 64, 2 + gates), dim3(256), 0, st, r);
+  }
+  return rsm::after_launch(call);
+}
+
+}  // extern "C"

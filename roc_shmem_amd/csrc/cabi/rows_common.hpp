@@ -1,0 +1,85 @@
+// Argument checks shared by the row collectives.
+#ifndef ROCSHMEM_MI355X_ROWS_COMMON_HPP
+#define ROCSHMEM_MI355X_ROWS_COMMON_HPP
+
+#include <string>
+#include <vector>
+
+#include "cabi_common.hpp"
+
+namespace rsm {
+
+// The members of a team, as the kernels address them: a symmetric pointer of PE 0 moved by `first`
+// bytes is the first member's copy, and every further `step` bytes the next member's.
+struct Members {
+  int size;
+  int64_t first, step;
+};
+
+// The symmetric operands of one call: every one has to lie in a live allocation, and none that the
+// call writes may share bytes with another, unless the two are one array on purpose.
+class Operands {
+ public:
+  explicit Operands(const char *call) : call_(call) {}
+
+  // rows x cols elements of `size` bytes, `ld` elements from row to row.
+  void matrix(const void *p, const char *name, size_t rows, size_t cols, size_t ld, size_t size, bool written) {
+    add(p, name, rows && cols ? ((rows - 1) * ld + cols) * size : 0, written);
+  }
+  void add(const void *p, const char *name, size_t bytes, bool written) {
+    if (p) spans_.push_back({static_cast<const char *>(p), bytes, name, written, nullptr});
+  }
+  // The operand added last may be the very array `p`: each row of `p` is read before it is written.
+  void or_same_as(const void *p) {
+    if (!spans_.empty() && spans_.back().p == p) spans_.back().same = p;
+  }
+
+  bool ok() const {
+    for (const Span &s : spans_) {
+      const std::string what = std::string(call_) + ": " + s.name;
+      if (!check_symmetric(s.p, what.c_str()) || !check_extent(s.p, s.bytes, what.c_str())) return false;
+    }
+    for (size_t i = 0; i < spans_.size(); ++i)
+      for (size_t j = 0; j < i; ++j) {
+        const Span &a = spans_[i], &b = spans_[j];
+        if (!(a.written || b.written) || !(a.p < b.p + b.bytes && b.p < a.p + a.bytes)) continue;
+        if (a.p == b.p && ((a.same == b.p && !b.written) || (b.same == a.p && !a.written))) continue;
+        fail(std::string(call_) + ": " + a.name + " and " + b.name + " overlap");
+        return false;
+      }
+    return true;
+  }
+
+ private:
+  struct Span {
+    const char *p;
+    size_t bytes;
+    const char *name;
+    bool written;
+    const void *same;
+  };
+  const char *call_;
+  std::vector<Span> spans_;
+};
+
+// False, with the error set, when `team` is none; otherwise its members.
+inline bool members_of(uint64_t team, const char *call, Members *out) {
+  rocshmem::host::Runtime *rt = rocshmem::host::Runtime::get();
+  if (!rt) {
+    fail("rsm_init has not been called");
+    return false;
+  }
+  const auto *rec = rt->team_record(reinterpret_cast<rocshmem::detail::Team *>(team));
+  if (!rec) {
+    fail(std::string(call) + ": invalid team");
+    return false;
+  }
+  const auto &t = rec->image.wrt_world;
+  const int64_t stride = static_cast<int64_t>(rt->slice_stride());
+  *out = {t.size, t.pe_start * stride, t.stride * stride};
+  return true;
+}
+
+}  // namespace rsm
+
+#endif

@@ -1,0 +1,149 @@
+// Building blocks of the row collectives (norm_to_all, logprob_to_all and their gradients): rows of
+// float or bfloat16 read and written 16 bytes per lane at any element alignment, held as float, and
+// sums over the lanes of a row.
+#ifndef ROCSHMEM_MI355X_DEVICE_ROWS_HPP
+#define ROCSHMEM_MI355X_DEVICE_ROWS_HPP
+
+#include <hip/hip_bf16.h>
+
+#include "copy.hpp"
+#include "reduce.hpp"
+#include "wave.hpp"
+
+namespace rocshmem {
+namespace detail {
+
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+
+// Elements of T in a 16-byte vector.
+template <typename T>
+constexpr int kRowVec = 16 / static_cast<int>(sizeof(T));
+
+// The kRowVec<T> elements at `p` as raw bits.  `left` elements of the row remain: the rest of the
+// vector is not read and comes back as `fill` bits.  A row may start at any element: the hardware
+// reads a 16-byte vector at any address (kTail false: `left` is a multiple of kRowVec<T>).
+template <typename T, bool kTail>
+__device__ __forceinline__ u32x4 row_load(const T *p, int left, uint32_t fill = 0) {
+  u32x4 v = {fill, fill, fill, fill};
+  if (!kTail ? left > 0 : left >= kRowVec<T>) {
+    v = *reinterpret_cast<const u32x4_a2 *>(p);
+  } else if (kTail && left > 0) {
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (e < left) v[e] = q[e];
+    } else {
+      const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (e < left)
+          v[e / 2] = e % 2 ? (v[e / 2] & 0xffffu) | static_cast<uint32_t>(q[e]) << 16
+                           : (v[e / 2] & 0xffff0000u) | q[e];
+    }
+  }
+  return v;
+}
+
+// Element e of a raw vector as float.
+template <typename T>
+__device__ __forceinline__ float row_get(u32x4 v, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(v[e]);
+  else return __uint_as_float(e % 2 ? v[e / 2] & 0xffff0000u : v[e / 2] << 16);
+}
+
+// Two floats rounded to bfloat16 (nearest even), the first in the low half.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+  const b16x2 b = __builtin_convertvector((f32x2{lo, hi}), b16x2);
+  return __builtin_bit_cast(uint32_t, b);
+}
+
+// Floats rounded once to T, as raw bits.
+template <typename T>
+__device__ __forceinline__ u32x4 row_pack(const float (&f)[kRowVec<T>]) {
+  u32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) v[k] = __float_as_uint(f[k]);
+    else v[k] = pack_bf16(f[2 * k], f[2 * k + 1]);
+  }
+  return v;
+}
+
+template <typename T, bool kTail>
+__device__ __forceinline__ void row_store(T *p, int left, u32x4 v) {
+  if (!kTail ? left > 0 : left >= kRowVec<T>) {
+    *reinterpret_cast<u32x4_a2 *>(p) = v;
+  } else if (kTail && left > 0) {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t *q = reinterpret_cast<uint32_t *>(p);
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (e < left) q[e] = v[e];
+    } else {
+      uint16_t *q = reinterpret_cast<uint16_t *>(p);
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (e < left) q[e] = static_cast<uint16_t>(e % 2 ? v[e / 2] >> 16 : v[e / 2]);
+    }
+  }
+}
+
+// `p` moved by `bytes`.
+template <typename T>
+__device__ __forceinline__ T *bytes_on(T *p, int64_t bytes) {
+  return reinterpret_cast<T *>(reinterpret_cast<uintptr_t>(p) + static_cast<uintptr_t>(bytes));
+}
+
+// Value of `v` under a DPP control word; lanes the control leaves out get 0.
+template <int kCtrl, int kRowMask = 0xf>
+__device__ __forceinline__ float dpp_or_zero(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), kCtrl, kRowMask, 0xf, false));
+}
+
+// Sum over the 64 lanes, the same in every lane.  Within rows of 16 lanes by quad permutes and
+// rotations, then row 0 into 1 and 2 into 3, then row 1 into 3: lane 63 holds the sum.  All in the
+// vector unit, without a trip through LDS for each of the six steps.
+__device__ __forceinline__ float wave_sum(float v) {
+  v += dpp_or_zero<0xB1>(v);         // quad_perm [1,0,3,2]
+  v += dpp_or_zero<0x4E>(v);         // quad_perm [2,3,0,1]
+  v += dpp_or_zero<0x124>(v);        // row_ror:4
+  v += dpp_or_zero<0x128>(v);        // row_ror:8
+  v += dpp_or_zero<0x142, 0xa>(v);   // row_bcast:15 into rows 1 and 3
+  v += dpp_or_zero<0x143, 0xc>(v);   // row_bcast:31 into rows 2 and 3
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+}
+
+// Sums of kN values over the kLanes lanes that hold a row (a wave, or the whole workgroup), the same
+// in every lane.  `slots` is LDS for 2 x (kLanes / 64) x kN floats and `turn` picks its half, which
+// alternates from call to call: a lane that writes the half again has passed the barrier of the call
+// in between, behind which nobody reads the older sums any more.
+template <int kLanes, int kN>
+__device__ __forceinline__ void row_sums(float (&v)[kN], float *slots, int &turn) {
+#pragma unroll
+  for (int k = 0; k < kN; ++k) v[k] = wave_sum(v[k]);
+  if constexpr (kLanes > 64) {
+    constexpr int kWaves = kLanes / 64;
+    float *mine = slots + turn * kWaves * kN;
+    turn ^= 1;
+    if (lane_id() == 0) {
+#pragma unroll
+      for (int k = 0; k < kN; ++k) mine[(threadIdx.x / 64) * kN + k] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) s += mine[w * kN + k];
+      v[k] = s;
+    }
+  }
+}
+
+}  // namespace detail
+}  // namespace rocshmem
+
+#endif
