@@ -40,7 +40,7 @@ struct LogprobForward {
   const char *logits;
   const int64_t *tokens;
   char *logprob, *entropy, *lse, *top_ids, *top_logprobs;
-  // A row is cut into batches (kBatch elements per lane group, never across members); workgroup
+  // A row is cut into batches (kBatch elements, never across members); workgroup
   // q of `parts` takes its share of them in order.
   int batches_per_member, parts;
   float4 *part_sums;     // [rows][parts]: m, l, w
@@ -121,9 +121,10 @@ __device__ __forceinline__ void top_offer(TopList &t, bool offered, float value,
   }
 }
 
-// One batch of a wave: `left` elements of the member's part from `p` on, the first of them id `id`.
-template <typename T, bool kTop>
-__device__ __forceinline__ void take_batch(const T *p, int left, int id, float c2, int top_k, Softmax &a, TopList &t) {
+// One batch of a wave: `left` elements of the member's part from `p` on.  Returns the largest of this
+// lane's elements.
+template <typename T>
+__device__ __forceinline__ float take_batch(const T *p, int left, float c2, Softmax &a) {
   constexpr int V = kRowVec<T>;
   constexpr uint32_t kMinusInf = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
   const int lane = lane_id();
@@ -147,18 +148,74 @@ __device__ __forceinline__ void take_batch(const T *p, int left, int id, float c
       a.l += f;
       a.w = fmaf(f, fmaxf(d, kFarBelow), a.w);
     }
-  if constexpr (kTop) {
-    // Ids grow from batch to batch, so an equal value in a later batch never beats the list once it is full.
-    if (__ballot(best > t.last_value || t.last_id == kNoId)) {
+  return best;
+}
+
+// ---- the likeliest alternatives -----------------------------------------------------------------
+//
+// While it streams, a lane notes the largest element of every batch.  The k-th largest of 64 disjoint
+// groups' maxima is a bound that at least k elements of the row reach, and few more: with 64 groups
+// and k = 20 some 24.  Only batches whose noted maximum reaches the bound are read again (from the
+// caches), their elements above it are gathered in LDS, and one wave ranks them by (value, id).  The
+// price per logit is nothing but the maximum that the softmax needs anyway.  Rows in which more than
+// kMaxFound elements reach the bound (equal values, or fewer numbers than k) are gone through once
+// more in ascending order of ids, batch by batch, into a sorted list.
+
+constexpr int kMaxFound = 256, kNotes = 16;
+
+// Orders floats as unsigned numbers.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// A value, in 16 bits' precision and not above it, that the k largest of the lanes' values reach; minus
+// infinity where fewer than k do.
+__device__ __forceinline__ float bound_of_lanes(float v, int k) {
+  const uint32_t key = order_of(v);
+  uint32_t bound = 0;
 #pragma unroll
-      for (int k = 0; k < kDeep; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int c = (k * 64 + lane) * V + e;
-          top_offer(t, c < left, row_get<T>(raw[k], e), id + c, top_k);
-        }
-    }
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t with = bound | 1u << bit;
+    if (__popcll(__ballot(key >= with)) >= k) bound = with;
   }
+  const uint32_t u = bound & 0x80000000u ? bound & 0x7fffffffu : ~bound;
+  return bound <= 0x007fffffu ? -INFINITY : __uint_as_float(u);   // below: minus infinity and NaN
+}
+
+struct Found {
+  int count;
+  float value[kMaxFound];
+  int id[kMaxFound];
+};
+
+__device__ __forceinline__ void found_add(Found &f, float value, int id) {
+  const int at = atomicAdd(&f.count, 1);
+  if (at < kMaxFound) {
+    f.value[at] = value;
+    f.id[at] = id;
+  }
+}
+
+// The best of what was found, sorted, by one wave.
+__device__ __forceinline__ TopList found_best(const Found &f, int n, int top_k) {
+  TopList t;
+  top_clear(t);
+  const int lane = lane_id();
+  if (n > 64) {
+    for (int i = 0; i < n; i += 64)
+      top_offer(t, i + lane < n, i + lane < n ? f.value[i + lane] : 0.f, i + lane < n ? f.id[i + lane] : 0, top_k);
+    return t;
+  }
+  const float v = lane < n ? f.value[lane] : -INFINITY;
+  const int id = lane < n ? f.id[lane] : kNoId;
+  int rank = 0;
+  for (int i = 0; i < n; ++i) rank += beats(lane_value(v, i), static_cast<int>(__builtin_amdgcn_readlane(id, i)), v, id);
+  if (lane >= n) rank = lane;
+  // every lane sends its element to the lane of its rank
+  t.value = __uint_as_float(__builtin_amdgcn_ds_permute(rank * 4, __float_as_uint(v)));
+  t.id = __builtin_amdgcn_ds_permute(rank * 4, id);
+  return t;
 }
 
 template <typename T>
@@ -170,20 +227,19 @@ __device__ __forceinline__ float logit_of(const LogprobForward &p, int row, int6
 }
 
 // Writes a row's results to every member; called by one whole wave.
-template <typename T, bool kTop>
-__device__ __forceinline__ void finish_row(const LogprobForward &p, int row, Softmax a, TopList t, float c2) {
+template <bool kTop>
+__device__ __forceinline__ void finish_row(const LogprobForward &p, int row, Softmax a, TopList t, int64_t token, float of_token) {
   const int lane = lane_id();
   const float log_l = log2f(a.l) * kLn2;
   const bool empty = a.l == 0.f;   // no logit above minus infinity
   const float lse = empty ? -INFINITY : fmaf(p.scale, a.m, log_l);
   const float entropy = empty ? 0.f : fmaf(-kLn2, a.w / a.l, log_l);
   float logprob = 0.f;
-  const int64_t token = p.tokens ? p.tokens[row] : -1;
   if (token >= p.vocab) {
     if (lane == 0) status_raise(kStatusBadArgument);
     logprob = NAN;
   } else if (token >= 0) {
-    logprob = empty ? -INFINITY : fmaf(p.scale, logit_of<T>(p, row, token) - a.m, -log_l);
+    logprob = empty ? -INFINITY : fmaf(p.scale, of_token - a.m, -log_l);
   }
   for (int m = lane; m < p.members; m += 64) {
     if (p.logprob) reinterpret_cast<float *>(p.logprob + m * p.step)[row] = logprob;
@@ -206,54 +262,132 @@ __device__ __forceinline__ void finish_row(const LogprobForward &p, int row, Sof
 
 constexpr int kMaxWaves = 8;
 
+// Where a batch of a row lies: its first element, how many there are, and the first one's id.
+template <typename T>
+struct Batch {
+  const T *p;
+  int left, id;
+};
+template <typename T>
+__device__ __forceinline__ Batch<T> batch_at(const LogprobForward &p, int row, int b) {
+  const int member = uniform(b / p.batches_per_member);
+  const int at = (b - member * p.batches_per_member) * kBatch<T>;
+  const int64_t id = static_cast<int64_t>(member) * p.shard + at;
+  int left = p.shard - at;
+  if (id + left > p.vocab) left = id < p.vocab ? static_cast<int>(p.vocab - id) : 0;
+  return {reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at, left, static_cast<int>(id)};
+}
+
+template <typename T>
+__device__ __forceinline__ float element_at(const Batch<T> &b, int c) {
+  if constexpr (sizeof(T) == 4) return c < b.left ? b.p[c] : -INFINITY;
+  else return c < b.left ? bf16_bits_to_float(reinterpret_cast<const uint16_t *>(b.p)[c]) : -INFINITY;
+}
+
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kMaxWaves * 64) logprob_kernel(LogprobForward p) {
   __shared__ Softmax sums[kMaxWaves];
-  __shared__ float values[kMaxWaves][kMaxTop];
-  __shared__ int ids[kMaxWaves][kMaxTop];
+  __shared__ float lane_best[kTop ? kMaxWaves : 1][64];
+  __shared__ float notes[kTop ? kMaxWaves : 1][kNotes][64];
+  __shared__ Found found;
   const int lane = lane_id(), wave = uniform(static_cast<int>(threadIdx.x / 64)), waves = blockDim.x / 64;
   const int row = uniform(static_cast<int>(blockIdx.x / p.parts)), part = uniform(static_cast<int>(blockIdx.x % p.parts));
   const float c2 = p.scale * kLog2e;
+  // the token's logit, long before it is needed
+  int64_t token = -1;
+  float of_token = 0.f;
+  if (wave == 0 && p.logprob) {
+    token = p.tokens[row];
+    if (token >= 0 && token < p.vocab) of_token = logit_of<T>(p, row, token);
+  }
+  if (kTop && threadIdx.x == 0) found.count = 0;
   Softmax a{kLowest, 0.f, 0.f};
-  TopList t;
-  top_clear(t);
   const int64_t batches = static_cast<int64_t>(p.batches_per_member) * p.members;
   const int first = static_cast<int>(batches * part / p.parts), end = static_cast<int>(batches * (part + 1) / p.parts);
+  // batches of this wave that share a note
+  const int per_note = ((end - first + waves - 1) / waves + kNotes - 1) / kNotes;
+  float best = -INFINITY, note = -INFINITY;
+  int turn = 0, at_note = 0;
   for (int b = first + wave; b < end; b += waves) {
-    const int member = uniform(b / p.batches_per_member);
-    const int at = (b - member * p.batches_per_member) * kBatch<T>;
-    const int64_t id = static_cast<int64_t>(member) * p.shard + at;
-    int left = p.shard - at;
-    if (id + left > p.vocab) left = id < p.vocab ? static_cast<int>(p.vocab - id) : 0;
-    if (left <= 0) continue;
-    const T *x = reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at;
-    take_batch<T, kTop>(x, left, static_cast<int>(id), c2, p.top_k, a, t);
-  }
-  a = join_lanes(a, c2);
-  if (waves > 1) {
-    if (lane == 0) sums[wave] = a;
+    const Batch<T> batch = batch_at<T>(p, row, b);
+    const float here = take_batch<T>(batch.p, batch.left, c2, a);
     if constexpr (kTop) {
-      if (lane < p.top_k) {
-        values[wave][lane] = t.value;
-        ids[wave][lane] = t.id;
+      best = fmaxf(best, here);
+      note = fmaxf(note, here);
+      notes[wave][at_note][lane] = note;
+      if (++turn == per_note) {
+        turn = 0;
+        ++at_note;
+        note = -INFINITY;
       }
     }
+  }
+  a = join_lanes(a, c2);
+  TopList t;
+  top_clear(t);
+  if (kTop || waves > 1) {
+    if (lane == 0) sums[wave] = a;
+    if constexpr (kTop) lane_best[wave][lane] = best;
     __syncthreads();
+    if constexpr (kTop) {
+      for (int w = 0; w < waves; ++w) best = fmaxf(best, lane_best[w][lane]);
+      const float bound = bound_of_lanes(best, p.top_k);
+      if (bound != -INFINITY) {
+        turn = at_note = 0;
+        for (int b = first + wave; b < end; b += waves) {
+          const bool near = notes[wave][at_note][lane] >= bound;
+          if (++turn == per_note) {
+            turn = 0;
+            ++at_note;
+          }
+          if (!__ballot(near) || *const_cast<volatile int *>(&found.count) > kMaxFound) continue;
+          const Batch<T> batch = batch_at<T>(p, row, b);
+          if (!near) continue;
+          u32x4 raw[kDeep];
+#pragma unroll
+          for (int k = 0; k < kDeep; ++k) {
+            const int c = (k * 64 + lane) * kRowVec<T>;
+            raw[k] = row_load<T, true>(batch.p + c, batch.left - c, sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u);
+          }
+#pragma unroll
+          for (int k = 0; k < kDeep; ++k)
+#pragma unroll
+            for (int e = 0; e < kRowVec<T>; ++e) {
+              const float x = row_get<T>(raw[k], e);
+              if (x >= bound) found_add(found, x, batch.id + (k * 64 + lane) * kRowVec<T> + e);
+            }
+        }
+      }
+      __syncthreads();
+      if (wave != 0) return;
+      if (bound != -INFINITY && found.count <= kMaxFound) {
+        t = found_best(found, uniform(found.count), p.top_k);
+      } else {
+        for (int b = first; b < end; ++b) {
+          const int w = (b - first) % waves, i = (b - first) / waves;
+          const float noted = notes[w][i / per_note][lane];
+          // ids grow from batch to batch: an equal value never beats a full list
+          if (!__ballot(noted > t.last_value || t.last_id == kNoId)) continue;
+          const Batch<T> batch = batch_at<T>(p, row, b);
+          for (int e = 0; e < kBatch<T> / 64; ++e) {
+            const int c = e * 64 + lane;
+            top_offer(t, c < batch.left, element_at(batch, c), batch.id + c, p.top_k);
+          }
+        }
+      }
+    }
     if (wave != 0) return;
     a = lane < waves ? sums[lane] : Softmax{kLowest, 0.f, 0.f};
     a = join_lanes(a, c2);
-    if constexpr (kTop) {
-      for (int w = 1; w < waves; ++w)
-        top_offer(t, lane < p.top_k && ids[w][lane] != kNoId, values[w][lane % kMaxTop], ids[w][lane % kMaxTop], p.top_k);
-    }
   }
   if (p.parts == 1) {
-    finish_row<T, kTop>(p, row, a, t, c2);
+    finish_row<kTop>(p, row, a, t, token, of_token);
     return;
   }
-  // The workgroups of a row leave what they have; the one that arrives last joins it.  The words go
-  // past the L2 of the XCD (agent-scope stores), the writer waits for them, and only then counts
-  // itself in; the last one reads them the same way.
+  // The workgroups of a row leave what they have; the one that arrives last joins it.  The words are
+  // written past the L2 of the XCD (agent-scope stores), the writer waits for them, and only then counts
+  // itself in; the last one reads them with agent-scope loads behind its count.  A release of the whole
+  // L2 is not needed for them.
   const int64_t at = static_cast<int64_t>(row) * p.parts + part;
   float *mine = reinterpret_cast<float *>(p.part_sums + at);
   auto leave = [](auto *to, auto v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
@@ -265,30 +399,50 @@ __global__ void __launch_bounds__(kMaxWaves * 64) logprob_kernel(LogprobForward 
       leave(p.part_ids + at * p.top_k + lane, t.id);
     }
   }
-  fence_release_agent();
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
   unsigned before = 0;
   if (lane == 0) before = __hip_atomic_fetch_add(p.arrived + 2 * row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (uniform(before) != static_cast<unsigned>(p.parts - 1)) return;
-  fence_acquire_agent();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   if (lane == 0) leave(p.arrived + 2 * row, 0u);
   a = {kLowest, 0.f, 0.f};
   for (int q = lane; q < p.parts; q += 64) {
     float *theirs = reinterpret_cast<float *>(p.part_sums + static_cast<int64_t>(row) * p.parts + q);
     a = join(a, {fetch(theirs), fetch(theirs + 1), fetch(theirs + 2)}, c2);
   }
-  a = join_lanes(a, c2);
   if constexpr (kTop) {
-    top_clear(t);
-    const int64_t theirs = static_cast<int64_t>(row) * p.parts * p.top_k;
+    // the same bound over the parts' lists
+    float *values = p.part_values + static_cast<int64_t>(row) * p.parts * p.top_k;
+    int *theirs = p.part_ids + static_cast<int64_t>(row) * p.parts * p.top_k;
     const int n = p.parts * p.top_k;
-    for (int i = 0; i < n; i += 64) {
-      const bool there = i + lane < n;
-      const float v = there ? fetch(p.part_values + theirs + i + lane) : -INFINITY;
-      const int id = there ? fetch(p.part_ids + theirs + i + lane) : kNoId;
-      top_offer(t, id != kNoId, v, id, p.top_k);
+    best = -INFINITY;
+    for (int i = lane; i < n; i += 64) best = fmaxf(best, fetch(values + i));
+    const float bound = bound_of_lanes(best, p.top_k);
+    if (lane == 0) found.count = 0;
+    __builtin_amdgcn_wave_barrier();
+    if (bound != -INFINITY) {
+      for (int i = lane; i < n; i += 64) {
+        const float v = fetch(values + i);
+        if (v >= bound) found_add(found, v, fetch(theirs + i));
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    const int all = uniform(*const_cast<volatile int *>(&found.count));
+    if (bound != -INFINITY && all <= kMaxFound) {
+      t = found_best(found, all, p.top_k);
+    } else {
+      top_clear(t);
+      for (int i = 0; i < n; i += 64) {
+        const bool there = i + lane < n;
+        const float v = there ? fetch(values + i + lane) : -INFINITY;
+        const int id = there ? fetch(theirs + i + lane) : kNoId;
+        top_offer(t, id != kNoId, v, id, p.top_k);
+      }
     }
   }
-  finish_row<T, kTop>(p, row, a, t, c2);
+  a = join_lanes(a, c2);
+  finish_row<kTop>(p, row, a, t, token, of_token);
 }
 
 struct LogprobBackward {
