@@ -73,10 +73,8 @@ __device__ __forceinline__ Softmax join(Softmax a, Softmax b, float c2) {
 }
 
 __device__ __forceinline__ Softmax join_lanes(Softmax a, float c2) {
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2)
-    a = join(a, {__shfl_xor(a.m, k), __shfl_xor(a.l, k), __shfl_xor(a.w, k)}, c2);
-  return a;
+  lift(a, wave_max(a.m), c2);
+  return {a.m, wave_sum(a.l), wave_sum(a.w)};
 }
 
 // The best elements seen so far by a wave: lane r holds the one of rank r.
@@ -123,7 +121,7 @@ __device__ __forceinline__ void top_offer(TopList &t, bool offered, float value,
 
 // One batch of a wave: `left` elements of the member's part from `p` on.  Returns the largest of this
 // lane's elements.
-template <typename T>
+template <typename T, bool kNt>
 __device__ __forceinline__ float take_batch(const T *p, int left, float c2, Softmax &a) {
   constexpr int V = kRowVec<T>;
   constexpr uint32_t kMinusInf = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
@@ -132,7 +130,7 @@ __device__ __forceinline__ float take_batch(const T *p, int left, float c2, Soft
 #pragma unroll
   for (int k = 0; k < kDeep; ++k) {
     const int c = (k * 64 + lane) * V;
-    raw[k] = row_load<T, true>(p + c, left - c, kMinusInf);
+    raw[k] = row_load<T, true, kNt>(p + c, left - c, kMinusInf);
   }
   float best = -INFINITY;
 #pragma unroll
@@ -260,7 +258,7 @@ __device__ __forceinline__ void finish_row(const LogprobForward &p, int row, Sof
   }
 }
 
-constexpr int kMaxWaves = 8;
+constexpr int kMaxWaves = 8, kMaxParts = 16;
 
 // Where a batch of a row lies: its first element, how many there are, and the first one's id.
 template <typename T>
@@ -284,8 +282,10 @@ __device__ __forceinline__ float element_at(const Batch<T> &b, int c) {
   else return c < b.left ? bf16_bits_to_float(reinterpret_cast<const uint16_t *>(b.p)[c]) : -INFINITY;
 }
 
-template <typename T, bool kTop>
-__global__ void __launch_bounds__(kMaxWaves * 64) logprob_kernel(LogprobForward p) {
+// 64 vector registers at most, so that a compute unit holds four workgroups: while some rank their
+// row's alternatives the others stream.
+template <typename T, bool kTop, bool kNt>
+__global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForward p) {
   __shared__ Softmax sums[kMaxWaves];
   __shared__ float lane_best[kTop ? kMaxWaves : 1][64];
   __shared__ float notes[kTop ? kMaxWaves : 1][kNotes][64];
@@ -293,13 +293,7 @@ __global__ void __launch_bounds__(kMaxWaves * 64) logprob_kernel(LogprobForward 
   const int lane = lane_id(), wave = uniform(static_cast<int>(threadIdx.x / 64)), waves = blockDim.x / 64;
   const int row = uniform(static_cast<int>(blockIdx.x / p.parts)), part = uniform(static_cast<int>(blockIdx.x % p.parts));
   const float c2 = p.scale * kLog2e;
-  // the token's logit, long before it is needed
-  int64_t token = -1;
-  float of_token = 0.f;
-  if (wave == 0 && p.logprob) {
-    token = p.tokens[row];
-    if (token >= 0 && token < p.vocab) of_token = logit_of<T>(p, row, token);
-  }
+  const int64_t token = p.logprob ? p.tokens[row] : -1;
   if (kTop && threadIdx.x == 0) found.count = 0;
   Softmax a{kLowest, 0.f, 0.f};
   const int64_t batches = static_cast<int64_t>(p.batches_per_member) * p.members;
@@ -310,7 +304,7 @@ __global__ void __launch_bounds__(kMaxWaves * 64) logprob_kernel(LogprobForward 
   int turn = 0, at_note = 0;
   for (int b = first + wave; b < end; b += waves) {
     const Batch<T> batch = batch_at<T>(p, row, b);
-    const float here = take_batch<T>(batch.p, batch.left, c2, a);
+    const float here = take_batch<T, kNt>(batch.p, batch.left, c2, a);
     if constexpr (kTop) {
       best = fmaxf(best, here);
       note = fmaxf(note, here);
@@ -322,6 +316,9 @@ __global__ void __launch_bounds__(kMaxWaves * 64) logprob_kernel(LogprobForward 
       }
     }
   }
+  // the token's logit, before what follows needs it
+  float of_token = 0.f;
+  if (wave == 0 && token >= 0 && token < p.vocab) of_token = logit_of<T>(p, row, token);
   a = join_lanes(a, c2);
   TopList t;
   top_clear(t);
@@ -407,25 +404,37 @@ __global__ void __launch_bounds__(kMaxWaves * 64) logprob_kernel(LogprobForward 
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   if (lane == 0) leave(p.arrived + 2 * row, 0u);
   a = {kLowest, 0.f, 0.f};
-  for (int q = lane; q < p.parts; q += 64) {
-    float *theirs = reinterpret_cast<float *>(p.part_sums + static_cast<int64_t>(row) * p.parts + q);
-    a = join(a, {fetch(theirs), fetch(theirs + 1), fetch(theirs + 2)}, c2);
+  if (lane < p.parts) {
+    float *theirs = reinterpret_cast<float *>(p.part_sums + static_cast<int64_t>(row) * p.parts + lane);
+    a = {fetch(theirs), fetch(theirs + 1), fetch(theirs + 2)};
   }
   if constexpr (kTop) {
-    // the same bound over the parts' lists
-    float *values = p.part_values + static_cast<int64_t>(row) * p.parts * p.top_k;
-    int *theirs = p.part_ids + static_cast<int64_t>(row) * p.parts * p.top_k;
+    // the same bound over the parts' lists, all of them in registers
+    constexpr int kHeld = kMaxParts * kMaxTop / 64;
+    const int64_t lists = static_cast<int64_t>(row) * p.parts * p.top_k;
     const int n = p.parts * p.top_k;
+    float v[kHeld];
+    int id[kHeld];
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int i = k * 64 + lane;
+      v[k] = -INFINITY;
+      id[k] = kNoId;
+      if (i < n) {
+        v[k] = fetch(p.part_values + lists + i);
+        id[k] = fetch(p.part_ids + lists + i);
+      }
+    }
     best = -INFINITY;
-    for (int i = lane; i < n; i += 64) best = fmaxf(best, fetch(values + i));
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) best = fmaxf(best, v[k]);
     const float bound = bound_of_lanes(best, p.top_k);
     if (lane == 0) found.count = 0;
     __builtin_amdgcn_wave_barrier();
     if (bound != -INFINITY) {
-      for (int i = lane; i < n; i += 64) {
-        const float v = fetch(values + i);
-        if (v >= bound) found_add(found, v, fetch(theirs + i));
-      }
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if (v[k] >= bound) found_add(found, v[k], id[k]);
     }
     __builtin_amdgcn_wave_barrier();
     const int all = uniform(*const_cast<volatile int *>(&found.count));
@@ -433,11 +442,12 @@ __global__ void __launch_bounds__(kMaxWaves * 64) logprob_kernel(LogprobForward 
       t = found_best(found, all, p.top_k);
     } else {
       top_clear(t);
-      for (int i = 0; i < n; i += 64) {
-        const bool there = i + lane < n;
-        const float v = there ? fetch(values + i + lane) : -INFINITY;
-        const int id = there ? fetch(theirs + i + lane) : kNoId;
-        top_offer(t, id != kNoId, v, id, p.top_k);
+#pragma unroll 1
+      for (int k = 0; k < kHeld; ++k) {
+        const int i = k * 64 + lane;
+        const float value = i < n ? fetch(p.part_values + lists + i) : -INFINITY;
+        const int name = i < n ? fetch(p.part_ids + lists + i) : kNoId;
+        top_offer(t, name != kNoId, value, name, p.top_k);
       }
     }
   }
@@ -553,13 +563,14 @@ LogprobPlan plan_of(const LogprobShape &s, int dtype, size_t rows, size_t vocab,
   g.batches = static_cast<int>((width_of(s, vocab) + batch - 1) / batch);
   const int64_t all = static_cast<int64_t>(g.batches) * s.team.size;
   g.parts = 1;
-  // few rows: several workgroups to a row, so that the chip has some 512 to run, each with a wave's
-  // batch at least
+  // Few rows: several workgroups to a row, so that the chip has some 512 to run, each with a batch for
+  // each of its waves.  More and smaller ones lose more in the joining than they win (one row of 128000
+  // bf16 with 20 alternatives: 8 workgroups of 8 waves 14.7 us, 16 of 4 15.3, 32 of 2 18.1, 64 of 1 24).
   if (rows && rows < 256) {
     int64_t parts = 512 / static_cast<int64_t>(rows);
-    const int64_t most = (all + 1) / 2;
+    const int64_t most = (all + kMaxWaves - 1) / kMaxWaves;
     if (parts > most) parts = most;
-    if (parts > 64) parts = 64;
+    if (parts > kMaxParts) parts = kMaxParts;
     g.parts = parts < 1 ? 1 : static_cast<int>(parts);
   }
   const int64_t mine = (all + g.parts - 1) / g.parts;
@@ -573,6 +584,17 @@ char *moved(void *p, int64_t bytes) { return p ? static_cast<char *>(p) + bytes 
 template <typename T>
 const T *moved_as(const void *p, int64_t bytes) {
   return reinterpret_cast<const T *>(moved(p, bytes));
+}
+
+template <typename T>
+void launch_forward(const LogprobForward &p, dim3 grid, dim3 block, hipStream_t st, bool once) {
+  if (p.top_k) {
+    if (once) hipLaunchKernelGGL((logprob_kernel<T, true, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((logprob_kernel<T, true, false>), grid, block, 0, st, p);
+  } else {
+    if (once) hipLaunchKernelGGL((logprob_kernel<T, false, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((logprob_kernel<T, false, false>), grid, block, 0, st, p);
+  }
 }
 
 bool top_in_range(const char *call, int top_k, size_t vocab) {
@@ -651,13 +673,11 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
   }
   const dim3 grid(static_cast<unsigned>(a.rows * g.parts)), block(static_cast<unsigned>(g.waves * 64));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (a.dtype == RSM_BF16) {
-    if (a.top_k) hipLaunchKernelGGL((logprob_kernel<__hip_bfloat16, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((logprob_kernel<__hip_bfloat16, false>), grid, block, 0, st, p);
-  } else {
-    if (a.top_k) hipLaunchKernelGGL((logprob_kernel<float, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((logprob_kernel<float, false>), grid, block, 0, st, p);
-  }
+  // Logits that the Infinity Cache could not hold anyway are read past it: 4096 x 131072 bf16 without
+  // alternatives 168 us against 186; smaller ones may still lie there from the product that made them.
+  const bool once = a.rows * a.vocab * size > rsm::kInfinityCacheBytes;
+  if (a.dtype == RSM_BF16) launch_forward<__hip_bfloat16>(p, grid, block, st, once);
+  else launch_forward<float>(p, grid, block, st, once);
   return rsm::after_launch(call);
 }
 

@@ -9,6 +9,9 @@
 
 namespace rsm {
 
+// What the MI355X's last-level cache holds.
+constexpr size_t kInfinityCacheBytes = 256u << 20;
+
 // The members of a team, as the kernels address them: a symmetric pointer of PE 0 moved by `first`
 // bytes is the first member's copy, and every further `step` bytes the next member's.
 struct Members {

@@ -22,11 +22,13 @@ constexpr int kRowVec = 16 / static_cast<int>(sizeof(T));
 // The kRowVec<T> elements at `p` as raw bits.  `left` elements of the row remain: the rest of the
 // vector is not read and comes back as `fill` bits.  A row may start at any element: the hardware
 // reads a 16-byte vector at any address (kTail false: `left` is a multiple of kRowVec<T>).
-template <typename T, bool kTail>
+// kNt: past the caches' allocation, for data that is read once and would not stay in them.
+template <typename T, bool kTail, bool kNt = false>
 __device__ __forceinline__ u32x4 row_load(const T *p, int left, uint32_t fill = 0) {
   u32x4 v = {fill, fill, fill, fill};
   if (!kTail ? left > 0 : left >= kRowVec<T>) {
-    v = *reinterpret_cast<const u32x4_a2 *>(p);
+    if constexpr (kNt) v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a2 *>(p));
+    else v = *reinterpret_cast<const u32x4_a2 *>(p);
   } else if (kTail && left > 0) {
     if constexpr (sizeof(T) == 4) {
       const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
@@ -113,6 +115,20 @@ __device__ __forceinline__ float wave_sum(float v) {
   v += dpp_or_zero<0x128>(v);        // row_ror:8
   v += dpp_or_zero<0x142, 0xa>(v);   // row_bcast:15 into rows 1 and 3
   v += dpp_or_zero<0x143, 0xc>(v);   // row_bcast:31 into rows 2 and 3
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+}
+
+// Largest of the lanes' values, the same in every lane; none of them is NaN.
+__device__ __forceinline__ float wave_max(float v) {
+#define RSM_MAX_STEP(ctrl, rows)                                                                       \
+  v = fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(v), __float_as_uint(v), ctrl, rows, 0xf, false)))
+  RSM_MAX_STEP(0xB1, 0xf);
+  RSM_MAX_STEP(0x4E, 0xf);
+  RSM_MAX_STEP(0x124, 0xf);
+  RSM_MAX_STEP(0x128, 0xf);
+  RSM_MAX_STEP(0x142, 0xa);
+  RSM_MAX_STEP(0x143, 0xc);
+#undef RSM_MAX_STEP
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
 }
 

@@ -163,7 +163,8 @@ def logprob_forward(logits, tokens, scale, top_k):
 
 def logprob_backward(logits, tokens, lse, entropy, scale, g_logprob, g_entropy, g_lse):
     """(value, error) of the gradient of the logits, from the lse and entropy given.  exp(lp) is off by 3
-    roundings of lp and 2 of its own, the factor behind it by 6."""
+    roundings of lp and 2 of its own, the factor behind it by 6; and a probability below the smallest
+    normal number, 2^-126, may be taken for 0, which leaves out 2^-126 times that factor."""
     rows, vocab = logits.shape
     col = lambda v: np.zeros((rows, 1)) if v is None else np.asarray(v, dtype=np.float64)[:, None]  # noqa: E731
     with np.errstate(all="ignore"):
@@ -174,9 +175,10 @@ def logprob_backward(logits, tokens, lse, entropy, scale, g_logprob, g_entropy, 
         ge, gs, h = col(g_entropy), col(g_lse), col(entropy)
         inner = np.where(p == 0, 0, lp)
         d = p * (gs - gl - ge * (inner + h))
-        d_abs = p * (np.abs(gs) + np.abs(gl) + np.abs(ge) * (np.abs(inner) + np.abs(h)))
+        factor = np.abs(gs) + np.abs(gl) + np.abs(ge) * (np.abs(inner) + np.abs(h))
+        d_abs = p * factor
         if tokens is not None:
             hit = np.arange(vocab)[None, :] == tokens[:, None]
             d = d + np.where(hit, gl, 0)
             d_abs = d_abs + np.where(hit, np.abs(gl), 0)
-        return d * scale, U32 * scale * d_abs * (14 + 3 * np.abs(inner))
+        return d * scale, U32 * scale * d_abs * (14 + 3 * np.abs(inner)) + scale * 2.0 ** -126 * factor

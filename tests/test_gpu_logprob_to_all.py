@@ -158,11 +158,10 @@ def test_backward_over_shapes(dtype, rows, vocab, pes, more):
         run_backward(Case(dtype, rows, vocab, pes, seed=rows + vocab, **more))
 
 
-@pytest.mark.parametrize("rows", [3, 300])
+@pytest.mark.parametrize("rows,vocab", [(3, 5000), (300, 5000), (2, 70001)])   # the last: several workgroups to a row
 @pytest.mark.parametrize("dtype", [rs.BF16, rs.FLOAT])
-def test_masks(dtype, rows):
+def test_masks(dtype, rows, vocab):
     """Rows with few logits left, one, none; ties everywhere; rows at the type's lowest value."""
-    vocab = 5000
     rng = np.random.default_rng(rows)
     base = rng.standard_normal((rows, vocab)) * 2
     lowest = -3.3895314e38
@@ -202,15 +201,14 @@ def test_rows_at_the_lowest_value_are_uniform():
         assert np.array_equal(out["top_ids"].read(0), [[0, 1, 2]] * rows)
 
 
-@pytest.mark.parametrize("rows", [4, 400])
-def test_not_a_number(rows):
+@pytest.mark.parametrize("rows,vocab", [(4, 2500), (400, 2500), (4, 50000)])
+def test_not_a_number(rows, vocab):
     """A row with a NaN or plus infinity has NaN results, its neighbours have their own; NaN is never an
     alternative."""
-    vocab = 2500
     rng = np.random.default_rng(5)
     logits = rng.standard_normal((rows, vocab)).astype(np.float32)
     logits[1, 1234] = np.nan
-    logits[2, 2499] = np.inf
+    logits[2, vocab - 1] = np.inf
     logits[3] = np.nan
     with runtime(2):
         c = Case(rs.FLOAT, rows, vocab, 2, logits=logits, tokens=np.full(rows, 7), top_k=4)
@@ -223,7 +221,7 @@ def test_not_a_number(rows):
         ids = out["top_ids"].read(0)
         order = lambda v: np.argsort(-v, kind="stable")[:4]  # noqa: E731
         assert np.array_equal(ids[1], order(np.where(np.isnan(logits[1]), -np.inf, logits[1])))
-        assert ids[2][0] == 2499
+        assert ids[2][0] == vocab - 1
         assert np.array_equal(ids[3], [-1] * 4) and np.isnan(out["top_logprobs"].read(0)[3]).all()
         lse = out["lse"].read(0)[0]
         g = Rows(rows, c.width, np.float32, c.ld)

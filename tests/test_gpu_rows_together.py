@@ -41,12 +41,12 @@ def test_operands_that_do_not_fit_or_overlap_are_refused():
         refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(**g), "work")
         refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(work=small, **g), "work")
         refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(work=source, **g), "overlap|fit")
-        d = LogprobCase(rs.FLOAT, 8, 1000, 4, top_k=3)
+        d = LogprobCase(rs.FLOAT, 8, 100000, 4, top_k=3)      # so few rows of so many share a workspace
         o = d.outputs()
         args = d.call(o)
         for change, word in [(dict(work=None), "work"), (dict(pSync=None), "pSync"), (dict(pSync=small), "pSync"),
-                             (dict(logits_ld=1 << 20), "logits"), (dict(lse=o["entropy"]), "overlap"),
-                             (dict(lse=d.array), "overlap|fit"), (dict(shard=200), "cover"), (dict(logits_ld=249), "stride"),
+                             (dict(logits_ld=1 << 22), "logits"), (dict(lse=o["entropy"]), "overlap"),
+                             (dict(lse=d.array), "overlap|fit"), (dict(shard=200), "cover"), (dict(logits_ld=24999), "stride"),
                              (dict(team=0), "team"), (dict(tokens=outside.addr), "symmetric")]:
             fields = dict(top_k=3, work=args.work, pSync=args.pSync, **{**d.fields, **o})
             refused(rs.roc_shmem_logprob_to_all, rs.LogprobArgs(**{**fields, **change}), word)
