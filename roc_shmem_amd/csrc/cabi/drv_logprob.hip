@@ -466,11 +466,14 @@ struct LogprobBackward {
   int chunks;   // workgroups per row of a member
 };
 
-constexpr int kGradLanes = 256;
+// Bound by memory: without its arithmetic the kernel takes as long (4096 x 131072 bf16, by process 354
+// or 382 us; 361 or 390 without arithmetic and 4 vectors per lane).  Eight vectors of a lane in flight:
+// 391 us against 397 with four; stores past the caches' allocation on top: 382.
+constexpr int kGradLanes = 256, kGradDeep = 8;
 template <typename T>
-constexpr int kGradChunk = kGradLanes * kRowVec<T> * kDeep;
+constexpr int kGradChunk = kGradLanes * kRowVec<T> * kGradDeep;
 
-template <typename T>
+template <typename T, bool kNt>
 __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(LogprobBackward p) {
   constexpr int V = kRowVec<T>;
   const uint64_t b = static_cast<uint64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
@@ -486,9 +489,9 @@ __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(LogprobBackwar
   const T *x = reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at;
   T *out = reinterpret_cast<T *>(p.grad_logits + member * p.step) + row * p.grad_ld + at;
   const int lane = threadIdx.x;
-  u32x4 raw[kDeep];
+  u32x4 raw[kGradDeep];
 #pragma unroll
-  for (int k = 0; k < kDeep; ++k) {
+  for (int k = 0; k < kGradDeep; ++k) {
     const int c = (k * kGradLanes + lane) * V;
     raw[k] = row_load<T, true>(x + c, left - c);
   }
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(LogprobBackwar
   const float flat = of_lse - of_token - (p.grad_entropy ? of_entropy * p.entropy[row] : 0.f);
   const int64_t hit = token - id;
 #pragma unroll
-  for (int k = 0; k < kDeep; ++k) {
+  for (int k = 0; k < kGradDeep; ++k) {
     const int c = (k * kGradLanes + lane) * V;
     float d[V];
 #pragma unroll
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(LogprobBackwar
       d[e] = exp2_of(lp * kLog2e) * fmaf(-of_entropy, fmaxf(lp, kFarBelow), flat);
       if (c + e == hit) d[e] += of_token;
     }
-    row_store<T, true>(out + c, left - c, row_pack<T>(d));
+    row_store<T, true, kNt>(out + c, left - c, row_pack<T>(d));
   }
 }
 
@@ -595,6 +598,12 @@ void launch_forward(const LogprobForward &p, dim3 grid, dim3 block, hipStream_t 
     if (once) hipLaunchKernelGGL((logprob_kernel<T, false, true>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((logprob_kernel<T, false, false>), grid, block, 0, st, p);
   }
+}
+
+template <typename T>
+void launch_backward(const LogprobBackward &p, dim3 grid, hipStream_t st, bool large) {
+  if (large) hipLaunchKernelGGL((logprob_grad_kernel<T, true>), grid, dim3(kGradLanes), 0, st, p);
+  else hipLaunchKernelGGL((logprob_grad_kernel<T, false>), grid, dim3(kGradLanes), 0, st, p);
 }
 
 bool top_in_range(const char *call, int top_k, size_t vocab) {
@@ -732,8 +741,9 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   if (y > 65535) return rsm::fail("logprob_to_all_grad: too many rows for one launch");
   const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(y));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (a.dtype == RSM_BF16) hipLaunchKernelGGL((logprob_grad_kernel<__hip_bfloat16>), grid, dim3(kGradLanes), 0, st, p);
-  else hipLaunchKernelGGL((logprob_grad_kernel<float>), grid, dim3(kGradLanes), 0, st, p);
+  const bool large = 2 * a.rows * a.vocab * size > rsm::kInfinityCacheBytes;
+  if (a.dtype == RSM_BF16) launch_backward<__hip_bfloat16>(p, grid, st, large);
+  else launch_backward<float>(p, grid, st, large);
   return rsm::after_launch(call);
 }
 

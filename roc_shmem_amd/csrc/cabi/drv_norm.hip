@@ -67,7 +67,7 @@ __device__ __forceinline__ T *row_at(char *base, int64_t bytes, int64_t row, int
 constexpr int kFoldDepth = 8;   // members whose loads are in flight together
 
 // Sum over the members of one row's elements that this lane holds.
-template <typename T, int kLanes, int NV, bool kTail>
+template <typename T, int kLanes, int NV, bool kTail, bool kNt>
 __device__ __forceinline__ void fold_members(const NormShape &s, const char *base, int64_t row, int64_t ld,
                                              int lane, float (&acc)[NV][kRowVec<T>]) {
   constexpr int V = kRowVec<T>;
@@ -84,7 +84,7 @@ __device__ __forceinline__ void fold_members(const NormShape &s, const char *bas
       for (int v = 0; v < NV; ++v) {
         const int c = (v * kLanes + lane) * V;
         raw[k][v] = u32x4{0u, 0u, 0u, 0u};
-        if (m + k < s.members) raw[k][v] = row_load<T, kTail>(row_at<T>(base, (m + k) * s.step, row, ld, c), s.cols - c);
+        if (m + k < s.members) raw[k][v] = row_load<T, kTail, kNt>(row_at<T>(base, (m + k) * s.step, row, ld, c), s.cols - c);
       }
     }
 #pragma unroll
@@ -96,12 +96,12 @@ __device__ __forceinline__ void fold_members(const NormShape &s, const char *bas
   }
 }
 
-template <typename T, int kLanes, int NV, bool kTail>
+template <typename T, int kLanes, int NV, bool kTail, bool kNt = false>
 __device__ __forceinline__ void load_row(const T *p, int cols, int lane, u32x4 (&raw)[NV]) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c = (v * kLanes + lane) * kRowVec<T>;
-    raw[v] = row_load<T, kTail>(p + c, cols - c);
+    raw[v] = row_load<T, kTail, kNt>(p + c, cols - c);
   }
 }
 
@@ -116,7 +116,7 @@ __device__ __forceinline__ void store_row(T *p, int64_t step, int copies, int co
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * kLanes + lane) * kRowVec<T>;
-      row_store<T, kTail>(bytes_on(p, m * step) + c, cols - c, raw[v]);
+      row_store<T, kTail, true>(bytes_on(p, m * step) + c, cols - c, raw[v]);
     }
   }
 }
@@ -124,7 +124,7 @@ __device__ __forceinline__ void store_row(T *p, int64_t step, int copies, int co
 template <int kLanes>
 constexpr int kWgLanes = kLanes < 256 ? 256 : kLanes;
 
-template <typename T, int kLanes, int NV, bool kTail>
+template <typename T, int kLanes, int NV, bool kTail, bool kNt>
 __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
   constexpr int V = kRowVec<T>;
   __shared__ float slots[2 * (kWgLanes<kLanes> / 64)];
@@ -138,14 +138,14 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
   const int64_t held = s.replicated ? row : row - owner * s.share;
 
   u32x4 x[NV], wpre[NV], wpost[NV], gate[NV];
-  load_row<T, kLanes, NV, kTail>(row_at<T>(p.residual, home, held, s.residual_ld, 0), s.cols, lane, x);
+  load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.residual, home, held, s.residual_ld, 0), s.cols, lane, x);
   if (p.pre_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, wpre);
   if (p.post_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.post_weight, home, 0, 0, 0), s.cols, lane, wpost);
   if (p.gate)
     load_row<T, kLanes, NV, kTail>(row_at<T>(p.gate, home, row / s.rows_per_gate, s.cols, 0), s.cols, lane, gate);
 
   float acc[NV][V];
-  fold_members<T, kLanes, NV, kTail>(s, p.source, row, s.partial_ld, lane, acc);
+  fold_members<T, kLanes, NV, kTail, kNt>(s, p.source, row, s.partial_ld, lane, acc);
   if (p.total) store_row<T, kLanes, NV, kTail>(row_at<T>(p.total, home, row - owner * s.share, s.cols, 0), 0, 1, s.cols, lane, acc);
 
   if (s.post) {
@@ -204,7 +204,7 @@ __device__ __forceinline__ void store_part(float *part, int64_t at, int ld, int 
   }
 }
 
-template <typename T, int kLanes, int NV, bool kTail>
+template <typename T, int kLanes, int NV, bool kTail, bool kNt>
 __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackward p) {
   constexpr int V = kRowVec<T>;
   __shared__ float slots[2 * 3 * (kWgLanes<kLanes> / 64)];
@@ -237,13 +237,13 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
     const int64_t held = s.replicated ? row : shared;
     const int gate_row = uniform(static_cast<int>(row) / s.rows_per_gate);
     u32x4 x[NV], tot[NV], din[NV], w[NV];
-    load_row<T, kLanes, NV, kTail>(row_at<T>(p.residual_out, home, held, s.residual_ld, 0), s.cols, lane, x);
-    if (p.total) load_row<T, kLanes, NV, kTail>(row_at<T>(p.total, home, shared, s.cols, 0), s.cols, lane, tot);
+    load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.residual_out, home, held, s.residual_ld, 0), s.cols, lane, x);
+    if (p.total) load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.total, home, shared, s.cols, 0), s.cols, lane, tot);
     if (p.grad_residual_out)
-      load_row<T, kLanes, NV, kTail>(row_at<T>(p.grad_residual_out, home, held, s.residual_ld, 0), s.cols, lane, din);
+      load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.grad_residual_out, home, held, s.residual_ld, 0), s.cols, lane, din);
     float d[NV][V];
     if (p.grad_normed) {
-      fold_members<T, kLanes, NV, kTail>(s, p.grad_normed, row, s.normed_ld, lane, d);
+      fold_members<T, kLanes, NV, kTail, kNt>(s, p.grad_normed, row, s.normed_ld, lane, d);
       if (p.pre_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, w);
     }
     // sum x'^2, sum t x' and sum s^2 in one go: the second mean is r(x') times a plain sum
@@ -340,9 +340,10 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
   if (p.part_gate) store_part<T, kLanes, NV>(p.part_gate, unit, p.part_ld, s.cols, lane, sum_gate);
 }
 
-// The units' sums, added up in ascending order of a fixed tree: workgroup (x, y) makes columns
-// 64 x .. 64 x + 63 of sum y (0: pre_weight, 1: post_weight, then the gate rows) and writes them to
-// every member.
+// The units' sums, added up in a fixed order: workgroup (x, y) makes columns 32 x .. 32 x + 31 of sum y
+// (0: pre_weight, 1: post_weight, then the gate rows) and writes them to every member.  32 columns, so
+// that two sums of 4096 columns already make 256 workgroups, with 32 lanes to share a column's units.
+constexpr int kSumQuads = 8, kSumRanks = 256 / kSumQuads;
 struct PartSums {
   const float *part_pre, *part_post, *part_gate;
   char *grad_pre, *grad_post, *grad_gate;
@@ -351,13 +352,13 @@ struct PartSums {
 };
 
 __global__ void __launch_bounds__(256) part_sums_kernel(PartSums p) {
-  __shared__ float4 sums[16][17];
+  __shared__ float4 sums[kSumRanks][kSumQuads];
   const int y = blockIdx.y;
   const float *part = y == 0 ? p.part_pre : y == 1 ? p.part_post : p.part_gate;
   char *out = y == 0 ? p.grad_pre : y == 1 ? p.grad_post : p.grad_gate;
   if (!out) return;
-  const int quad = threadIdx.x % 16, rank = threadIdx.x / 16;
-  const int c = (blockIdx.x * 16 + quad) * 4;
+  const int quad = threadIdx.x % kSumQuads, rank = threadIdx.x / kSumQuads;
+  const int c = (blockIdx.x * kSumQuads + quad) * 4;
   int first = 0, count = p.units;
   if (y >= 2) {
     first = (y - 2) * p.units_per_gate;
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(256) part_sums_kernel(PartSums p) {
   float4 sum{0.f, 0.f, 0.f, 0.f};
   if (c < p.cols) {
 #pragma unroll 8
-    for (int u = rank; u < count; u += 16) {
+    for (int u = rank; u < count; u += kSumRanks) {
       const float4 a = *reinterpret_cast<const float4 *>(part + static_cast<int64_t>(first + u) * p.part_ld + c);
       sum.x += a.x;
       sum.y += a.y;
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(256) part_sums_kernel(PartSums p) {
   sums[rank][quad] = sum;
   __syncthreads();
   if (rank != 0 || c >= p.cols) return;
-  for (int k = 1; k < 16; ++k) {
+  for (int k = 1; k < kSumRanks; ++k) {
     const float4 a = sums[k][quad];
     sum.x += a.x;
     sum.y += a.y;
@@ -400,46 +401,57 @@ struct RowLanes {
   int lanes, vecs;
 };
 RowLanes lanes_for(int cols, int vec) {
-  static const RowLanes choices[] = {{64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 1}, {512, 2}, {1024, 1}, {1024, 2}, {1024, 4}};
+  static const RowLanes choices[] = {{64, 1}, {64, 2}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
   for (const RowLanes &c : choices)
     if (c.lanes * c.vecs * vec >= cols) return c;
   return {0, 0};
 }
 
-template <typename T, int kLanes, int NV, typename P>
-void launch_rows(const P &p, int units, bool tail, hipStream_t stream) {
+template <typename T, int kLanes, int NV, typename P, bool kTail, bool kNt>
+void launch_rows(const P &p, int units, hipStream_t stream) {
   const unsigned per_wg = kWgLanes<kLanes> / kLanes;
   const dim3 grid((static_cast<unsigned>(units) + per_wg - 1) / per_wg), block(kWgLanes<kLanes>);
-  if constexpr (std::is_same<P, NormForward>::value) {
-    if (tail) hipLaunchKernelGGL((norm_kernel<T, kLanes, NV, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((norm_kernel<T, kLanes, NV, false>), grid, block, 0, stream, p);
+  if constexpr (std::is_same<P, NormForward>::value)
+    hipLaunchKernelGGL((norm_kernel<T, kLanes, NV, kTail, kNt>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((norm_grad_kernel<T, kLanes, NV, kTail, kNt>), grid, block, 0, stream, p);
+}
+
+// How a call goes: rows that end inside a vector, and operands that the Infinity Cache could not hold.
+struct Manner {
+  bool tail, once;
+};
+
+template <typename T, int kLanes, int NV, typename P>
+void launch_lanes(const P &p, int units, Manner m, hipStream_t stream) {
+  if (m.tail) {
+    if (m.once) launch_rows<T, kLanes, NV, P, true, true>(p, units, stream);
+    else launch_rows<T, kLanes, NV, P, true, false>(p, units, stream);
   } else {
-    if (tail) hipLaunchKernelGGL((norm_grad_kernel<T, kLanes, NV, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((norm_grad_kernel<T, kLanes, NV, false>), grid, block, 0, stream, p);
+    if (m.once) launch_rows<T, kLanes, NV, P, false, true>(p, units, stream);
+    else launch_rows<T, kLanes, NV, P, false, false>(p, units, stream);
   }
 }
 
 template <typename T, typename P>
-void launch_for(const P &p, int units, RowLanes l, hipStream_t stream) {
-  const bool tail = p.s.cols % kRowVec<T> != 0;
+void launch_for(const P &p, int units, RowLanes l, bool once, hipStream_t stream) {
+  const Manner m{p.s.cols % kRowVec<T> != 0, once};
   switch (l.lanes * 8 + l.vecs) {
-    case 64 * 8 + 1: launch_rows<T, 64, 1>(p, units, tail, stream); break;
-    case 64 * 8 + 2: launch_rows<T, 64, 2>(p, units, tail, stream); break;
-    case 256 * 8 + 1: launch_rows<T, 256, 1>(p, units, tail, stream); break;
-    case 256 * 8 + 2: launch_rows<T, 256, 2>(p, units, tail, stream); break;
-    case 512 * 8 + 1: launch_rows<T, 512, 1>(p, units, tail, stream); break;
-    case 512 * 8 + 2: launch_rows<T, 512, 2>(p, units, tail, stream); break;
-    case 1024 * 8 + 1: launch_rows<T, 1024, 1>(p, units, tail, stream); break;
-    case 1024 * 8 + 2: launch_rows<T, 1024, 2>(p, units, tail, stream); break;
+    case 64 * 8 + 1: launch_lanes<T, 64, 1>(p, units, m, stream); break;
+    case 64 * 8 + 2: launch_lanes<T, 64, 2>(p, units, m, stream); break;
+    case 256 * 8 + 1: launch_lanes<T, 256, 1>(p, units, m, stream); break;
+    case 512 * 8 + 1: launch_lanes<T, 512, 1>(p, units, m, stream); break;
+    case 1024 * 8 + 1: launch_lanes<T, 1024, 1>(p, units, m, stream); break;
+    case 1024 * 8 + 2: launch_lanes<T, 1024, 2>(p, units, m, stream); break;
     default:
-      if constexpr (sizeof(T) == 4) launch_rows<T, 1024, 4>(p, units, tail, stream);
+      if constexpr (sizeof(T) == 4) launch_lanes<T, 1024, 4>(p, units, m, stream);
   }
 }
 
 template <typename P>
-void launch_typed(int dtype, const P &p, int units, RowLanes l, hipStream_t stream) {
-  if (dtype == RSM_BF16) launch_for<__hip_bfloat16>(p, units, l, stream);
-  else launch_for<float>(p, units, l, stream);
+void launch_typed(int dtype, const P &p, int units, RowLanes l, bool once, hipStream_t stream) {
+  if (dtype == RSM_BF16) launch_for<__hip_bfloat16>(p, units, l, once, stream);
+  else launch_for<float>(p, units, l, once, stream);
 }
 
 size_t type_size(int dtype) { return dtype == RSM_FLOAT ? 4 : dtype == RSM_BF16 ? 2 : 0; }
@@ -525,6 +537,11 @@ GradPlan plan_of(const NormShape &s, int dtype, bool has_gate) {
   return g;
 }
 
+// What a call moves: every member's rows in and out, and `more` rows on the owners.
+size_t rows_bytes(const NormShape &s, size_t size, size_t more) {
+  return static_cast<size_t>(s.rows) * s.cols * size * (2 * static_cast<size_t>(s.members) + more);
+}
+
 const char *moved(const void *p, int64_t bytes) { return p ? static_cast<const char *>(p) + bytes : nullptr; }
 char *moved(void *p, int64_t bytes) { return p ? static_cast<char *>(p) + bytes : nullptr; }
 
@@ -567,7 +584,8 @@ int rsm_norm_to_all(const rsm_norm_args_t *args, void *stream) {
   p.residual_out = moved(a.residual_out, team.first);
   p.normed = moved(a.normed, team.first);
   p.total = moved(a.total, team.first);
-  launch_typed(a.dtype, p, s.rows, lanes_for(s.cols, a.dtype == RSM_BF16 ? 8 : 4), static_cast<hipStream_t>(stream));
+  launch_typed(a.dtype, p, s.rows, lanes_for(s.cols, a.dtype == RSM_BF16 ? 8 : 4),
+               rows_bytes(s, size, 2) > rsm::kInfinityCacheBytes, static_cast<hipStream_t>(stream));
   return rsm::after_launch(call);
 }
 
@@ -646,7 +664,7 @@ int rsm_norm_to_all_grad(const rsm_norm_grad_args_t *args, void *stream) {
   p.rows_per_unit = g.rows_per_unit;
   p.direct = g.direct;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (g.units) launch_typed(a.dtype, p, g.units, g.lanes, st);
+  if (g.units) launch_typed(a.dtype, p, g.units, g.lanes, rows_bytes(s, size, 4) > rsm::kInfinityCacheBytes, st);
   if (sums) {
     PartSums r{};
     r.part_pre = p.part_pre;
@@ -662,7 +680,7 @@ int rsm_norm_to_all_grad(const rsm_norm_grad_args_t *args, void *stream) {
     r.members = s.members;
     r.step = s.step;
     const unsigned gates = p.part_gate ? static_cast<unsigned>(gate_rows(s)) : 0;
-    hipLaunchKernelGGL(part_sums_kernel, dim3((s.cols + 63) / 64, 2 + gates), dim3(256), 0, st, r);
+    hipLaunchKernelGGL(part_sums_kernel, dim3((s.cols + 4 * kSumQuads - 1) / (4 * kSumQuads), 2 + gates), dim3(256), 0, st, r);
   }
   return rsm::after_launch(call);
 }

@@ -74,10 +74,11 @@ __device__ __forceinline__ u32x4 row_pack(const float (&f)[kRowVec<T>]) {
   return v;
 }
 
-template <typename T, bool kTail>
+template <typename T, bool kTail, bool kNt = false>
 __device__ __forceinline__ void row_store(T *p, int left, u32x4 v) {
   if (!kTail ? left > 0 : left >= kRowVec<T>) {
-    *reinterpret_cast<u32x4_a2 *>(p) = v;
+    if constexpr (kNt) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_a2 *>(p));
+    else *reinterpret_cast<u32x4_a2 *>(p) = v;
   } else if (kTail && left > 0) {
     if constexpr (sizeof(T) == 4) {
       uint32_t *q = reinterpret_cast<uint32_t *>(p);
