@@ -49,8 +49,9 @@ struct NormBackward {
   char *grad_source, *grad_residual, *grad_gate;
   float *part_pre, *part_post, *part_gate;   // [units][part_ld], null where nobody asks for them
   int part_ld;
-  // A unit (the lanes that hold a row) walks the rows of its own.  `direct`: whole gate groups,
-  // rows_per_unit of them a multiple of rows_per_gate; otherwise units_per_gate units share a group.
+  // A unit (the lanes that hold a row) walks rows of its own.  `direct`: rows_per_unit in a row, whole
+  // gate groups; otherwise units_per_gate units share a group and each takes every units_per_gate-th
+  // row of it, so that all units together sweep one compact window of every array.
   int units, units_per_gate, rows_per_unit;
   bool direct;
 };
@@ -209,43 +210,58 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
   constexpr int V = kRowVec<T>;
   __shared__ float slots[2 * 3 * (kWgLanes<kLanes> / 64)];
   __shared__ float slots1[2 * (kWgLanes<kLanes> / 64)];
+  // The sums of the two weights' gradients over the unit's rows, each lane's own: in LDS, since in
+  // registers they would halve the workgroups of a compute unit or, at 1024 lanes, spill.
+  __shared__ float4 sums_of[2][NV * V / 4][kWgLanes<kLanes>];
   int turn = 0, turn1 = 0;
   const NormShape &s = p.s;
   const int lane = threadIdx.x % kLanes;
   const int unit = uniform(static_cast<int>(blockIdx.x * (kWgLanes<kLanes> / kLanes) + threadIdx.x / kLanes));
   if (unit >= p.units) return;   // as in norm_kernel
-  int64_t first, last;
+  int64_t first, last, step = 1;
   if (p.direct) {
     first = static_cast<int64_t>(unit) * p.rows_per_unit;
     last = first + p.rows_per_unit;
   } else {
-    const int64_t group = unit / p.units_per_gate, end = (group + 1) * s.rows_per_gate;
-    first = group * s.rows_per_gate + static_cast<int64_t>(unit % p.units_per_gate) * p.rows_per_unit;
-    last = first + p.rows_per_unit < end ? first + p.rows_per_unit : end;
+    const int64_t group = unit / p.units_per_gate;
+    first = group * s.rows_per_gate + unit % p.units_per_gate;
+    last = (group + 1) * s.rows_per_gate;
+    step = p.units_per_gate;
   }
   if (last > s.rows) last = s.rows;
 
-  float sum_pre[NV][V], sum_post[NV][V], sum_gate[NV][V];
+  float sum_gate[NV][V];
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int e = 0; e < V; ++e) sum_pre[v][e] = sum_post[v][e] = sum_gate[v][e] = 0.f;
+    for (int e = 0; e < V; ++e) sum_gate[v][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV * V / 4; ++k) sums_of[0][k][threadIdx.x] = sums_of[1][k][threadIdx.x] = float4{0.f, 0.f, 0.f, 0.f};
+  // the weights' copies on the first member serve every row of the unit
+  u32x4 wpre[NV], wpost[NV];
+  if (p.pre_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.pre_weight, 0, 0, 0, 0), s.cols, lane, wpre);
+  if (p.post_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.post_weight, 0, 0, 0, 0), s.cols, lane, wpost);
 
-  for (int64_t row = first; row < last; ++row) {
+  auto add_to = [](auto &of, int v, const float (&f)[V]) {
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) {
+      float4 &sum = of[v * (V / 4) + k][threadIdx.x];
+      sum = float4{sum.x + f[4 * k], sum.y + f[4 * k + 1], sum.z + f[4 * k + 2], sum.w + f[4 * k + 3]};
+    }
+  };
+  for (int64_t row = first; row < last; row += step) {
     const int owner = uniform(static_cast<int>(row) / s.share);
     const int64_t home = owner * s.step, shared = row - static_cast<int64_t>(owner) * s.share;
     const int64_t held = s.replicated ? row : shared;
     const int gate_row = uniform(static_cast<int>(row) / s.rows_per_gate);
-    u32x4 x[NV], tot[NV], din[NV], w[NV];
+    u32x4 x[NV], tot[NV], din[NV], g[NV];
     load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.residual_out, home, held, s.residual_ld, 0), s.cols, lane, x);
     if (p.total) load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.total, home, shared, s.cols, 0), s.cols, lane, tot);
     if (p.grad_residual_out)
       load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.grad_residual_out, home, held, s.residual_ld, 0), s.cols, lane, din);
+    if (p.gate) load_row<T, kLanes, NV, kTail>(row_at<T>(p.gate, home, gate_row, s.cols, 0), s.cols, lane, g);
     float d[NV][V];
-    if (p.grad_normed) {
-      fold_members<T, kLanes, NV, kTail, kNt>(s, p.grad_normed, row, s.normed_ld, lane, d);
-      if (p.pre_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, w);
-    }
+    if (p.grad_normed) fold_members<T, kLanes, NV, kTail, kNt>(s, p.grad_normed, row, s.normed_ld, lane, d);
     // sum x'^2, sum t x' and sum s^2 in one go: the second mean is r(x') times a plain sum
     float sums[3] = {0.f, 0.f, 0.f};
 #pragma unroll
@@ -254,7 +270,7 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
       for (int e = 0; e < V; ++e) {
         if (p.grad_normed) {
           const float xe = row_get<T>(x[v], e);
-          const float t = d[v][e] * (p.pre_weight ? s.weight_offset + row_get<T>(w[v], e) : 1.f);
+          const float t = d[v][e] * (p.pre_weight ? s.weight_offset + row_get<T>(wpre[v], e) : 1.f);
           sums[0] = fmaf(xe, xe, sums[0]);
           sums[1] = fmaf(t, xe, sums[1]);
         }
@@ -265,18 +281,21 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
     const float mean_tn = sums[1] * r2 * s.inv_cols;
     const float r1 = rsqrtf(fmaf(sums[2], s.inv_cols, s.eps));
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      float to_pre[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float dd = p.grad_residual_out ? row_get<T>(din[v], e) : 0.f;
         if (p.grad_normed) {
           const float n = row_get<T>(x[v], e) * r2;
-          const float t = d[v][e] * (p.pre_weight ? s.weight_offset + row_get<T>(w[v], e) : 1.f);
-          sum_pre[v][e] = fmaf(d[v][e], n, sum_pre[v][e]);
+          const float t = d[v][e] * (p.pre_weight ? s.weight_offset + row_get<T>(wpre[v], e) : 1.f);
+          to_pre[e] = d[v][e] * n;
           dd = fmaf(r2, fmaf(-n, mean_tn, t), dd);
         }
         d[v][e] = dd;
       }
+      if (p.part_pre) add_to(sums_of[0], v, to_pre);
+    }
     if (p.grad_residual) {
       float dx[NV][V];
 #pragma unroll
@@ -287,28 +306,28 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
                                       s.replicated ? s.members : 1, s.cols, lane, dx);
     }
     // from here on d is f, and then q
-    u32x4 g[NV];
-    if (p.gate) load_row<T, kLanes, NV, kTail>(row_at<T>(p.gate, home, gate_row, s.cols, 0), s.cols, lane, g);
-    if (p.post_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.post_weight, home, 0, 0, 0), s.cols, lane, w);
     float qs[1] = {0.f};
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      float to_post[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float f = s.block_scale * d[v][e];
-        const float wp = p.post_weight ? s.weight_offset + row_get<T>(w[v], e) : 1.f;
+        const float wp = p.post_weight ? s.weight_offset + row_get<T>(wpost[v], e) : 1.f;
         const float u = p.total ? row_get<T>(tot[v], e) * (s.post ? r1 : 1.f) : 0.f;
         if (p.gate) {
           sum_gate[v][e] = fmaf(f, s.post ? u * wp : u, sum_gate[v][e]);
           f *= row_get<T>(g[v], e);
         }
         if (s.post) {
-          sum_post[v][e] = fmaf(f, u, sum_post[v][e]);
+          to_post[e] = f * u;
           f *= wp;
           qs[0] = fmaf(f, u, qs[0]);
         }
         d[v][e] = f;
       }
+      if (p.part_post) add_to(sums_of[1], v, to_post);
+    }
     if (s.post) {
       row_sums<kLanes>(qs, slots1, turn1);
       const float mean_qu = qs[0] * s.inv_cols;
@@ -335,8 +354,17 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
         for (int e = 0; e < V; ++e) sum_gate[v][e] = 0.f;
     }
   }
-  if (p.part_pre) store_part<T, kLanes, NV>(p.part_pre, unit, p.part_ld, s.cols, lane, sum_pre);
-  if (p.part_post) store_part<T, kLanes, NV>(p.part_post, unit, p.part_ld, s.cols, lane, sum_post);
+  auto leave = [&](float *part, auto &of) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) {
+        const int c = (v * kLanes + lane) * V + 4 * k;
+        if (c < s.cols) *reinterpret_cast<float4 *>(part + static_cast<int64_t>(unit) * p.part_ld + c) = of[v * (V / 4) + k][threadIdx.x];
+      }
+  };
+  if (p.part_pre) leave(p.part_pre, sums_of[0]);
+  if (p.part_post) leave(p.part_post, sums_of[1]);
   if (p.part_gate) store_part<T, kLanes, NV>(p.part_gate, unit, p.part_ld, s.cols, lane, sum_gate);
 }
 
