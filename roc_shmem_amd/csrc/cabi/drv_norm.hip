@@ -13,6 +13,7 @@
 //
 // Sums, means and everything between a load and a store are 32-bit floats; every output is rounded
 // to its type once.  Members are summed in ascending order, so every run gives the same bits.
+#include <cfloat>
 #include <cmath>
 
 #include "roc_shmem.hpp"
@@ -33,7 +34,8 @@ struct NormShape {
   int rows_per_gate;
   int64_t step;
   int64_t partial_ld, residual_ld, normed_ld;
-  float eps, inv_cols, residual_scale, block_scale, weight_offset;
+  float eps, inv_cols, residual_scale, block_scale;
+  float pre_offset, post_offset;    // what is added to the weights: weight_offset, or 1 where there are none
   bool post, replicated;
 };
 
@@ -65,19 +67,19 @@ __device__ __forceinline__ T *row_at(char *base, int64_t bytes, int64_t row, int
   return reinterpret_cast<T *>(base + bytes) + row * ld + col;
 }
 
-constexpr int kFoldDepth = 8;   // members whose loads are in flight together
+constexpr int kFoldDepth = 8;   // vectors of a lane, of several members, whose loads are in flight together
 
 // Sum over the members of one row's elements that this lane holds.
-template <typename T, int kLanes, int NV, bool kTail, bool kNt>
-__device__ __forceinline__ void fold_members(const NormShape &s, const char *base, int64_t row, int64_t ld,
+template <typename T, int kLanes, int NV, bool kTail, bool kNt, int kAtOnce = kFoldDepth>
+__device__ __forceinline__ void fold_members(const NormShape &s, int members, const char *base, int64_t row, int64_t ld,
                                              int lane, float (&acc)[NV][kRowVec<T>]) {
   constexpr int V = kRowVec<T>;
-  constexpr int kDepth = NV >= 4 ? 2 : NV == 2 ? 4 : kFoldDepth;
+  constexpr int kDepth = kAtOnce / NV < 1 ? 1 : kAtOnce / NV;
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[v][e] = 0.f;
-  for (int m = 0; m < s.members; m += kDepth) {
+  for (int m = 0; m < members; m += kDepth) {
     u32x4 raw[kDepth][NV];
 #pragma unroll
     for (int k = 0; k < kDepth; ++k) {
@@ -85,7 +87,7 @@ __device__ __forceinline__ void fold_members(const NormShape &s, const char *bas
       for (int v = 0; v < NV; ++v) {
         const int c = (v * kLanes + lane) * V;
         raw[k][v] = u32x4{0u, 0u, 0u, 0u};
-        if (m + k < s.members) raw[k][v] = row_load<T, kTail, kNt>(row_at<T>(base, (m + k) * s.step, row, ld, c), s.cols - c);
+        if (m + k < members) raw[k][v] = row_load<T, kTail, kNt>(row_at<T>(base, (m + k) * s.step, row, ld, c), s.cols - c);
       }
     }
 #pragma unroll
@@ -104,6 +106,29 @@ __device__ __forceinline__ void load_row(const T *p, int cols, int lane, u32x4 (
     const int c = (v * kLanes + lane) * kRowVec<T>;
     raw[v] = row_load<T, kTail, kNt>(p + c, cols - c);
   }
+}
+
+// A row that need not be there: elsewhere its elements have the bits `bits` stand for (0, or kOnes), so
+// that the arithmetic behind it asks no questions.
+template <typename T>
+constexpr uint32_t kOnes = sizeof(T) == 4 ? 0x3f800000u : 0x3f803f80u;
+template <typename T, int kLanes, int NV, bool kTail, bool kNt = false>
+__device__ __forceinline__ void load_row_or(bool there, uint32_t bits, const T *p, int cols, int lane, u32x4 (&raw)[NV]) {
+  if (there) {
+    load_row<T, kLanes, NV, kTail, kNt>(p, cols, lane, raw);
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) raw[v] = u32x4{bits, bits, bits, bits};
+  }
+}
+
+// Ends the life of everything derived from raw vectors: what follows unpacks them again.  Without it
+// the compiler carries the floats of bfloat16 rows, twice the registers, from one sum over the row to
+// what depends on it.
+template <int NV>
+__device__ __forceinline__ void keep_packed(u32x4 (&raw)[NV]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) __asm__ volatile("" : "+v"(raw[v]));
 }
 
 // The row to `copies` members, `step` bytes apart.
@@ -140,13 +165,13 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
 
   u32x4 x[NV], wpre[NV], wpost[NV], gate[NV];
   load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.residual, home, held, s.residual_ld, 0), s.cols, lane, x);
-  if (p.pre_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, wpre);
-  if (p.post_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.post_weight, home, 0, 0, 0), s.cols, lane, wpost);
-  if (p.gate)
-    load_row<T, kLanes, NV, kTail>(row_at<T>(p.gate, home, row / s.rows_per_gate, s.cols, 0), s.cols, lane, gate);
+  load_row_or<T, kLanes, NV, kTail>(p.pre_weight, 0u, row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, wpre);
+  load_row_or<T, kLanes, NV, kTail>(p.post_weight, 0u, row_at<T>(p.post_weight, home, 0, 0, 0), s.cols, lane, wpost);
+  load_row_or<T, kLanes, NV, kTail>(p.gate, kOnes<T>, row_at<T>(p.gate, home, row / s.rows_per_gate, s.cols, 0), s.cols,
+                                    lane, gate);
 
   float acc[NV][V];
-  fold_members<T, kLanes, NV, kTail, kNt>(s, p.source, row, s.partial_ld, lane, acc);
+  fold_members<T, kLanes, NV, kTail, kNt>(s, s.members, p.source, row, s.partial_ld, lane, acc);
   if (p.total) store_row<T, kLanes, NV, kTail>(row_at<T>(p.total, home, row - owner * s.share, s.cols, 0), 0, 1, s.cols, lane, acc);
 
   if (s.post) {
@@ -160,18 +185,14 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float w = p.post_weight ? s.weight_offset + row_get<T>(wpost[v], e) : 1.f;
-        acc[v][e] *= r * w;
-      }
+      for (int e = 0; e < V; ++e) acc[v][e] *= r * (s.post_offset + row_get<T>(wpost[v], e));
   }
   float ss[1] = {0.f};
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      float z = acc[v][e];
-      if (p.gate) z *= row_get<T>(gate[v], e);
+      const float z = acc[v][e] * row_get<T>(gate[v], e);
       acc[v][e] = fmaf(s.residual_scale, row_get<T>(x[v], e), s.block_scale * z);
       ss[0] = fmaf(acc[v][e], acc[v][e], ss[0]);
     }
@@ -183,10 +204,7 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float w = p.pre_weight ? s.weight_offset + row_get<T>(wpre[v], e) : 1.f;
-      acc[v][e] *= r * w;
-    }
+    for (int e = 0; e < V; ++e) acc[v][e] *= r * (s.pre_offset + row_get<T>(wpre[v], e));
   store_row<T, kLanes, NV, kTail>(row_at<T>(p.normed, 0, row, s.normed_ld, 0), s.step, s.members, s.cols, lane, acc);
 }
 
@@ -237,10 +255,21 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
     for (int e = 0; e < V; ++e) sum_gate[v][e] = 0.f;
 #pragma unroll
   for (int k = 0; k < NV * V / 4; ++k) sums_of[0][k][threadIdx.x] = sums_of[1][k][threadIdx.x] = float4{0.f, 0.f, 0.f, 0.f};
-  // the weights' copies on the first member serve every row of the unit
-  u32x4 wpre[NV], wpost[NV];
-  if (p.pre_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.pre_weight, 0, 0, 0, 0), s.cols, lane, wpre);
-  if (p.post_weight) load_row<T, kLanes, NV, kTail>(row_at<T>(p.post_weight, 0, 0, 0, 0), s.cols, lane, wpost);
+  // The weights' copies on the first member serve every row of the unit.  Rows of 16 elements to a lane
+  // (kTight) leave no registers for them: those loads are made again for every row, where the values are
+  // used, as is the gate's.
+  constexpr bool kTight = NV * V >= 16;
+  u32x4 wpre[NV], wpost[NV], g[NV];
+  auto load_pre = [&] {
+    load_row_or<T, kLanes, NV, kTail>(p.pre_weight, 0u, row_at<T>(p.pre_weight, 0, 0, 0, 0), s.cols, lane, wpre);
+  };
+  auto load_post = [&] {
+    load_row_or<T, kLanes, NV, kTail>(p.post_weight, 0u, row_at<T>(p.post_weight, 0, 0, 0, 0), s.cols, lane, wpost);
+  };
+  if constexpr (!kTight) {
+    load_pre();
+    load_post();
+  }
 
   auto add_to = [](auto &of, int v, const float (&f)[V]) {
 #pragma unroll
@@ -254,45 +283,48 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
     const int64_t home = owner * s.step, shared = row - static_cast<int64_t>(owner) * s.share;
     const int64_t held = s.replicated ? row : shared;
     const int gate_row = uniform(static_cast<int>(row) / s.rows_per_gate);
-    u32x4 x[NV], tot[NV], din[NV], g[NV];
-    load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.residual_out, home, held, s.residual_ld, 0), s.cols, lane, x);
-    if (p.total) load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.total, home, shared, s.cols, 0), s.cols, lane, tot);
-    if (p.grad_residual_out)
-      load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.grad_residual_out, home, held, s.residual_ld, 0), s.cols, lane, din);
-    if (p.gate) load_row<T, kLanes, NV, kTail>(row_at<T>(p.gate, home, gate_row, s.cols, 0), s.cols, lane, g);
+    u32x4 x[NV], tot[NV], din[NV];
+    load_row_or<T, kLanes, NV, kTail, kNt>(p.grad_normed, 0u, row_at<T>(p.residual_out, home, held, s.residual_ld, 0), s.cols,
+                                           lane, x);
+    load_row_or<T, kLanes, NV, kTail, kNt>(p.total, 0u, row_at<T>(p.total, home, shared, s.cols, 0), s.cols, lane, tot);
+    load_row_or<T, kLanes, NV, kTail, kNt>(p.grad_residual_out, 0u,
+                                           row_at<T>(p.grad_residual_out, home, held, s.residual_ld, 0), s.cols, lane, din);
+    auto load_gate = [&] {
+      load_row_or<T, kLanes, NV, kTail>(p.gate, kOnes<T>, row_at<T>(p.gate, home, gate_row, s.cols, 0), s.cols, lane, g);
+    };
+    if constexpr (!kTight) load_gate();
     float d[NV][V];
-    if (p.grad_normed) fold_members<T, kLanes, NV, kTail, kNt>(s, p.grad_normed, row, s.normed_ld, lane, d);
+    if constexpr (kTight) load_pre();
+    fold_members<T, kLanes, NV, kTail, kNt, kTight ? 4 : kFoldDepth>(s, p.grad_normed ? s.members : 0, p.grad_normed, row,
+                                                                    s.normed_ld, lane, d);
     // sum x'^2, sum t x' and sum s^2 in one go: the second mean is r(x') times a plain sum
     float sums[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        if (p.grad_normed) {
-          const float xe = row_get<T>(x[v], e);
-          const float t = d[v][e] * (p.pre_weight ? s.weight_offset + row_get<T>(wpre[v], e) : 1.f);
-          sums[0] = fmaf(xe, xe, sums[0]);
-          sums[1] = fmaf(t, xe, sums[1]);
-        }
-        if (s.post) sums[2] = fmaf(row_get<T>(tot[v], e), row_get<T>(tot[v], e), sums[2]);
+        const float xe = row_get<T>(x[v], e), se = row_get<T>(tot[v], e);
+        sums[0] = fmaf(xe, xe, sums[0]);
+        sums[1] = fmaf(d[v][e] * (s.pre_offset + row_get<T>(wpre[v], e)), xe, sums[1]);
+        sums[2] = fmaf(se, se, sums[2]);
       }
     row_sums<kLanes>(sums, slots, turn);
+    keep_packed(x);
+    keep_packed(tot);
+    keep_packed(din);
+    if constexpr (kTight) keep_packed(wpre);
     const float r2 = rsqrtf(fmaf(sums[0], s.inv_cols, s.eps));
     const float mean_tn = sums[1] * r2 * s.inv_cols;
-    const float r1 = rsqrtf(fmaf(sums[2], s.inv_cols, s.eps));
+    const float r1 = s.post ? rsqrtf(fmaf(sums[2], s.inv_cols, s.eps)) : 1.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float to_pre[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        float dd = p.grad_residual_out ? row_get<T>(din[v], e) : 0.f;
-        if (p.grad_normed) {
-          const float n = row_get<T>(x[v], e) * r2;
-          const float t = d[v][e] * (p.pre_weight ? s.weight_offset + row_get<T>(wpre[v], e) : 1.f);
-          to_pre[e] = d[v][e] * n;
-          dd = fmaf(r2, fmaf(-n, mean_tn, t), dd);
-        }
-        d[v][e] = dd;
+        const float n = row_get<T>(x[v], e) * r2;
+        const float t = d[v][e] * (s.pre_offset + row_get<T>(wpre[v], e));
+        to_pre[e] = d[v][e] * n;
+        d[v][e] = fmaf(r2, fmaf(-n, mean_tn, t), row_get<T>(din[v], e));
       }
       if (p.part_pre) add_to(sums_of[0], v, to_pre);
     }
@@ -306,30 +338,30 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
                                       s.replicated ? s.members : 1, s.cols, lane, dx);
     }
     // from here on d is f, and then q
+    if constexpr (kTight) {
+      load_gate();
+      load_post();
+    }
     float qs[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float to_post[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
+        const float w = s.post_offset + row_get<T>(wpost[v], e), u = row_get<T>(tot[v], e) * r1;
         float f = s.block_scale * d[v][e];
-        const float wp = p.post_weight ? s.weight_offset + row_get<T>(wpost[v], e) : 1.f;
-        const float u = p.total ? row_get<T>(tot[v], e) * (s.post ? r1 : 1.f) : 0.f;
-        if (p.gate) {
-          sum_gate[v][e] = fmaf(f, s.post ? u * wp : u, sum_gate[v][e]);
-          f *= row_get<T>(g[v], e);
-        }
-        if (s.post) {
-          to_post[e] = f * u;
-          f *= wp;
-          qs[0] = fmaf(f, u, qs[0]);
-        }
+        sum_gate[v][e] = fmaf(f, u * w, sum_gate[v][e]);
+        f *= row_get<T>(g[v], e);
+        to_post[e] = f * u;
+        f *= w;
+        qs[0] = fmaf(f, u, qs[0]);
         d[v][e] = f;
       }
       if (p.part_post) add_to(sums_of[1], v, to_post);
     }
     if (s.post) {
       row_sums<kLanes>(qs, slots1, turn1);
+      keep_packed(tot);
       const float mean_qu = qs[0] * s.inv_cols;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
@@ -424,15 +456,19 @@ __global__ void __launch_bounds__(256) part_sums_kernel(PartSums p) {
 
 // ---- host side ------------------------------------------------------------------------------------
 
-// Lanes per row and vectors per lane: the fewest of either that hold the row.
+// Lanes per row and vectors per lane: the fewest of either that hold the row.  The backward pass holds
+// several rows at a time; at 1024 lanes a compute unit has room for one workgroup of it, so 512 lanes
+// with more vectors come before.
 struct RowLanes {
   int lanes, vecs;
 };
-RowLanes lanes_for(int cols, int vec) {
-  static const RowLanes choices[] = {{64, 1}, {64, 2}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
-  for (const RowLanes &c : choices)
-    if (c.lanes * c.vecs * vec >= cols) return c;
-  return {0, 0};
+RowLanes lanes_for(int cols, int vec, bool backward) {
+  static const RowLanes forward_choices[] = {{64, 1}, {64, 2}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
+  static const RowLanes backward_bf16[] = {{64, 1}, {64, 2}, {256, 1}, {512, 1}, {512, 2}, {1024, 2}};
+  static const RowLanes backward_float[] = {{64, 1}, {64, 2}, {256, 1}, {512, 1}, {1024, 1}, {512, 4}, {1024, 4}};
+  const RowLanes *c = !backward ? forward_choices : vec == 8 ? backward_bf16 : backward_float;
+  while (c->lanes * c->vecs * vec < cols) ++c;   // the last of each holds kMaxCols elements
+  return *c;
 }
 
 template <typename T, int kLanes, int NV, typename P, bool kTail, bool kNt>
@@ -464,15 +500,26 @@ void launch_lanes(const P &p, int units, Manner m, hipStream_t stream) {
 template <typename T, typename P>
 void launch_for(const P &p, int units, RowLanes l, bool once, hipStream_t stream) {
   const Manner m{p.s.cols % kRowVec<T> != 0, once};
+  constexpr bool kBackward = std::is_same<P, NormBackward>::value, kBf16 = sizeof(T) == 2;
   switch (l.lanes * 8 + l.vecs) {
-    case 64 * 8 + 1: launch_lanes<T, 64, 1>(p, units, m, stream); break;
-    case 64 * 8 + 2: launch_lanes<T, 64, 2>(p, units, m, stream); break;
-    case 256 * 8 + 1: launch_lanes<T, 256, 1>(p, units, m, stream); break;
-    case 512 * 8 + 1: launch_lanes<T, 512, 1>(p, units, m, stream); break;
-    case 1024 * 8 + 1: launch_lanes<T, 1024, 1>(p, units, m, stream); break;
-    case 1024 * 8 + 2: launch_lanes<T, 1024, 2>(p, units, m, stream); break;
+    case 64 * 8 + 1: return launch_lanes<T, 64, 1>(p, units, m, stream);
+    case 64 * 8 + 2: return launch_lanes<T, 64, 2>(p, units, m, stream);
+    case 256 * 8 + 1: return launch_lanes<T, 256, 1>(p, units, m, stream);
+    case 512 * 8 + 1: return launch_lanes<T, 512, 1>(p, units, m, stream);
+    case 512 * 8 + 2:
+      if constexpr (kBackward && kBf16) return launch_lanes<T, 512, 2>(p, units, m, stream);
+      break;
+    case 512 * 8 + 4:
+      if constexpr (kBackward && !kBf16) return launch_lanes<T, 512, 4>(p, units, m, stream);
+      break;
+    case 1024 * 8 + 1:
+      if constexpr (!kBackward || !kBf16) return launch_lanes<T, 1024, 1>(p, units, m, stream);
+      break;
+    case 1024 * 8 + 2:
+      if constexpr (!kBackward || kBf16) return launch_lanes<T, 1024, 2>(p, units, m, stream);
+      break;
     default:
-      if constexpr (sizeof(T) == 4) launch_lanes<T, 1024, 4>(p, units, m, stream);
+      if constexpr (!kBf16) return launch_lanes<T, 1024, 4>(p, units, m, stream);
   }
 }
 
@@ -501,7 +548,7 @@ bool shape_of(const A &a, const char *call, size_t partial_ld, size_t normed_ld,
   const size_t far = ~size_t{0} >> 24;
   if (partial_ld > far / (a.rows + 1) || normed_ld > far / (a.rows + 1) || a.residual_ld > far / (a.rows + 1))
     return refuse("a row stride is too long");
-  if (!(a.eps > 0.f) || !std::isfinite(a.eps)) return refuse("eps must be a positive number");
+  if (!(a.eps >= FLT_MIN) || !std::isfinite(a.eps)) return refuse("eps must be a positive (normal) number");
   if (!std::isfinite(a.residual_scale) || !std::isfinite(a.block_scale) || !std::isfinite(a.weight_offset))
     return refuse("scales and the weight offset must be finite");
   if (a.post_weight && !(a.flags & RSM_NORM_POST)) return refuse("post_weight without RSM_NORM_POST");
@@ -522,7 +569,8 @@ bool shape_of(const A &a, const char *call, size_t partial_ld, size_t normed_ld,
   s.inv_cols = static_cast<float>(1.0 / static_cast<double>(a.cols));
   s.residual_scale = a.residual_scale;
   s.block_scale = a.block_scale;
-  s.weight_offset = a.weight_offset;
+  s.pre_offset = a.pre_weight ? a.weight_offset : 1.f;
+  s.post_offset = a.post_weight ? a.weight_offset : 1.f;
   s.post = (a.flags & RSM_NORM_POST) != 0;
   s.replicated = (a.flags & RSM_NORM_REPLICATED) != 0;
   *out = s;
@@ -542,7 +590,7 @@ struct GradPlan {
 
 GradPlan plan_of(const NormShape &s, int dtype, bool has_gate) {
   GradPlan g{};
-  g.lanes = lanes_for(s.cols, dtype == RSM_BF16 ? 8 : 4);
+  g.lanes = lanes_for(s.cols, dtype == RSM_BF16 ? 8 : 4, true);
   // enough units to fill the chip's 256 compute units, no more: each leaves its sums behind
   const int64_t target = g.lanes.lanes == 64 ? 4096 : 256 * (1024 / g.lanes.lanes);
   const int64_t per_unit = (s.rows + target - 1) / target;
@@ -612,7 +660,7 @@ int rsm_norm_to_all(const rsm_norm_args_t *args, void *stream) {
   p.residual_out = moved(a.residual_out, team.first);
   p.normed = moved(a.normed, team.first);
   p.total = moved(a.total, team.first);
-  launch_typed(a.dtype, p, s.rows, lanes_for(s.cols, a.dtype == RSM_BF16 ? 8 : 4),
+  launch_typed(a.dtype, p, s.rows, lanes_for(s.cols, a.dtype == RSM_BF16 ? 8 : 4, false),
                rows_bytes(s, size, 2) > rsm::kInfinityCacheBytes, static_cast<hipStream_t>(stream));
   return rsm::after_launch(call);
 }

@@ -94,10 +94,11 @@ __device__ __forceinline__ void row_store(T *p, int left, u32x4 v) {
   }
 }
 
-// `p` moved by `bytes`.
+// `p` moved by `bytes`.  Pointer arithmetic: an address that has been an integer is one of the flat
+// address space to the compiler, and flat stores share the counter that LDS results are waited for on.
 template <typename T>
 __device__ __forceinline__ T *bytes_on(T *p, int64_t bytes) {
-  return reinterpret_cast<T *>(reinterpret_cast<uintptr_t>(p) + static_cast<uintptr_t>(bytes));
+  return reinterpret_cast<T *>(reinterpret_cast<char *>(p) + bytes);
 }
 
 // Value of `v` under a DPP control word; lanes the control leaves out get 0.
