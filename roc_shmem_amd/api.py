@@ -400,8 +400,18 @@ def roc_shmem_small_ops(ops_dev, n_ops, fetched_dev=None, launch=None):
 from ._lib import LogprobArgs, LogprobGradArgs, NormArgs, NormGradArgs  # noqa: E402
 
 
+_row_entries = {}
+
+
+def _row_entry(name):
+    """The bound entry point, looked up once: a call of few rows takes the GPU about as long as Python."""
+    _row_entries[name] = entry = getattr(L.load(), name)
+    return entry
+
+
 def _row_call(name, args, stream):
-    _check(getattr(L.load(), name)(args, getattr(stream, "h", stream)))
+    if (_row_entries.get(name) or _row_entry(name))(args, stream.h if isinstance(stream, Stream) else stream):
+        _check(-1)
 
 
 def _row_bytes(name, args):

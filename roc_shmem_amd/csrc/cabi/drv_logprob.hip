@@ -29,9 +29,10 @@ constexpr int kMaxTop = 32;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kFarBelow = -200.f;        // 2^-200 is 0 as a float: stands for minus infinity in products
-constexpr int kNoId = 0x7fffffff;
 
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+
+constexpr int kMaxWaves = 8, kMaxParts = 16;
 
 struct LogprobForward {
   int rows, vocab, shard, members, top_k;
@@ -44,8 +45,7 @@ struct LogprobForward {
   // q of `parts` takes its share of them in order.
   int batches_per_member, parts;
   float4 *part_sums;     // [rows][parts]: m, l, w
-  float *part_values;    // [rows][parts][top_k]
-  int *part_ids;
+  uint64_t *part_keys;   // [rows][parts][top_k]
   unsigned *arrived;     // [rows], a 64-bit word apart, 0 on entry and on return
 };
 
@@ -77,60 +77,21 @@ __device__ __forceinline__ Softmax join_lanes(Softmax a, float c2) {
   return {a.m, wave_sum(a.l), wave_sum(a.w)};
 }
 
-// The best elements seen so far by a wave: lane r holds the one of rank r.
-struct TopList {
-  float value;
-  int id;
-  float last_value;   // the element of rank top_k - 1, the same in every lane: what another must beat
-  int last_id;
-};
-
-__device__ __forceinline__ float lane_value(float v, int lane) {
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
-}
-
-__device__ __forceinline__ bool beats(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
-
-__device__ __forceinline__ void top_clear(TopList &t) {
-  t.value = t.last_value = -INFINITY;
-  t.id = t.last_id = kNoId;
-}
-
-// One more element, the same in every lane.
-__device__ __forceinline__ void top_insert(TopList &t, float value, int id, int top_k) {
-  if (!beats(value, id, t.last_value, t.last_id)) return;
-  const int rank = __popcll(__ballot(beats(t.value, t.id, value, id)));
-  const float up_value = __uint_as_float(from_lower_lane(__float_as_uint(t.value)));
-  const int up_id = static_cast<int>(from_lower_lane(static_cast<uint32_t>(t.id)));
-  const int lane = lane_id();
-  t.value = lane > rank ? up_value : lane == rank ? value : t.value;
-  t.id = lane > rank ? up_id : lane == rank ? id : t.id;
-  t.last_value = lane_value(t.value, top_k - 1);
-  t.last_id = static_cast<int>(__builtin_amdgcn_readlane(t.id, top_k - 1));
-}
-
-// Every lane offers one element (`offered` false: none).
-__device__ __forceinline__ void top_offer(TopList &t, bool offered, float value, int id, int top_k) {
-  uint64_t mask = __ballot(offered && beats(value, id, t.last_value, t.last_id));
-  while (mask) {
-    const int lane = __builtin_ctzll(mask);
-    mask &= mask - 1;
-    top_insert(t, lane_value(value, lane), static_cast<int>(__builtin_amdgcn_readlane(id, lane)), top_k);
-  }
-}
+// Minus infinity in every element of a 32-bit word.
+template <typename T>
+constexpr uint32_t kMinusInf = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 
 // One batch of a wave: `left` elements of the member's part from `p` on.  Returns the largest of this
 // lane's elements.
 template <typename T, bool kNt>
 __device__ __forceinline__ float take_batch(const T *p, int left, float c2, Softmax &a) {
   constexpr int V = kRowVec<T>;
-  constexpr uint32_t kMinusInf = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
   const int lane = lane_id();
   u32x4 raw[kDeep];
 #pragma unroll
   for (int k = 0; k < kDeep; ++k) {
     const int c = (k * 64 + lane) * V;
-    raw[k] = row_load<T, true, kNt>(p + c, left - c, kMinusInf);
+    raw[k] = row_load<T, true, kNt>(p + c, left - c, kMinusInf<T>);
   }
   float best = -INFINITY;
 #pragma unroll
@@ -154,65 +115,108 @@ __device__ __forceinline__ float take_batch(const T *p, int left, float c2, Soft
 // While it streams, a lane notes the largest element of every batch.  The k-th largest of 64 disjoint
 // groups' maxima is a bound that at least k elements of the row reach, and few more: with 64 groups
 // and k = 20 some 24.  Only batches whose noted maximum reaches the bound are read again (from the
-// caches), their elements above it are gathered in LDS, and one wave ranks them by (value, id).  The
-// price per logit is nothing but the maximum that the softmax needs anyway.  Rows in which more than
-// kMaxFound elements reach the bound (equal values, or fewer numbers than k) are gone through once
-// more in ascending order of ids, batch by batch, into a sorted list.
+// caches), their elements above it are gathered in LDS, and one wave ranks them.  The price per logit
+// is nothing but the maximum that the softmax needs anyway.  Rows of which a wave finds more than
+// kRoom elements (equal values, or fewer numbers than k) are gone through once more in ascending
+// order of ids, batch by batch, into a sorted list.
+//
+// An element is a 64-bit key: its value, ordered as an unsigned number, above its id counted down, so
+// that the larger of two keys is the larger value or, of equal ones, the lower id; 0 is no element.
+typedef uint64_t Key;
+constexpr int kRoom = 64, kNotes = 16;
 
-constexpr int kMaxFound = 256, kNotes = 16;
-
-// Orders floats as unsigned numbers.
 __device__ __forceinline__ uint32_t order_of(float v) {
   const uint32_t u = __float_as_uint(v);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float value_of_order(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ Key key_of(float v, int id) {
+  return static_cast<Key>(order_of(v + 0.f)) << 32 | ~static_cast<uint32_t>(id);   // -0 equals 0
+}
+__device__ __forceinline__ float value_of(Key k) { return value_of_order(static_cast<uint32_t>(k >> 32)); }
+__device__ __forceinline__ int id_of(Key k) { return static_cast<int>(~static_cast<uint32_t>(k)); }
+__device__ __forceinline__ Key lane_key(Key k, int lane) {
+  return static_cast<Key>(__builtin_amdgcn_readlane(static_cast<uint32_t>(k >> 32), lane)) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(k), lane));
+}
 
-// A value, in 16 bits' precision and not above it, that the k largest of the lanes' values reach; minus
-// infinity where fewer than k do.
-__device__ __forceinline__ float bound_of_lanes(float v, int k) {
-  const uint32_t key = order_of(v);
+// The order of a value, in 16 bits and not above it, that the k largest of the lanes' orders reach.
+__device__ __forceinline__ uint32_t bound_of_lanes(uint32_t order, int k) {
   uint32_t bound = 0;
 #pragma unroll
   for (int bit = 31; bit >= 16; --bit) {
     const uint32_t with = bound | 1u << bit;
-    if (__popcll(__ballot(key >= with)) >= k) bound = with;
+    if (__popcll(__ballot(order >= with)) >= k) bound = with;
   }
-  const uint32_t u = bound & 0x80000000u ? bound & 0x7fffffffu : ~bound;
-  return bound <= 0x007fffffu ? -INFINITY : __uint_as_float(u);   // below: minus infinity and NaN
+  return bound;
 }
+constexpr uint32_t kOrderOfMinusInf = 0x007fffffu;   // what is not above it bounds nothing
 
-struct Found {
-  int count;
-  float value[kMaxFound];
-  int id[kMaxFound];
+// A wave's best elements in a sorted list: lane r holds the one of rank r.
+struct TopList {
+  Key key;
+  Key last;   // the element of rank top_k - 1, the same in every lane: what another must beat
 };
 
-__device__ __forceinline__ void found_add(Found &f, float value, int id) {
-  const int at = atomicAdd(&f.count, 1);
-  if (at < kMaxFound) {
-    f.value[at] = value;
-    f.id[at] = id;
+// Every lane offers one element (0: none).
+__device__ __forceinline__ void top_offer(TopList &t, Key offered, int top_k) {
+  uint64_t mask = __ballot(offered > t.last);
+  while (mask) {
+    const Key key = lane_key(offered, __builtin_ctzll(mask));
+    mask &= mask - 1;
+    if (key <= t.last) continue;
+    const int rank = __popcll(__ballot(t.key > key)), lane = lane_id();
+    const Key up = from_lower_lane(t.key);
+    t.key = lane > rank ? up : lane == rank ? key : t.key;
+    t.last = lane_key(t.key, top_k - 1);
   }
 }
 
-// The best of what was found, sorted, by one wave.
-__device__ __forceinline__ TopList found_best(const Found &f, int n, int top_k) {
-  TopList t;
-  top_clear(t);
+// Elements gathered by waves: each has room of its own, in LDS.
+struct Found {
+  Key key[kMaxWaves][kRoom];
+  int count[kMaxWaves];
+  Key all[64];
+};
+
+// Appends the lanes' elements (hit: there is one) to a wave's; `n` counts on beyond the room.
+__device__ __forceinline__ void found_add(Found &f, int wave, int &n, bool hit, Key key) {
+  const uint64_t mask = __ballot(hit);
+  if (mask == 0) return;
+  const int at = n + rank_in_mask(mask);
+  if (hit && at < kRoom) f.key[wave][at] = key;
+  n += __popcll(mask);
+}
+
+// What `waves` waves found, at most kRoom each, sorted by one wave.
+__device__ __forceinline__ TopList found_best(Found &f, int waves, int top_k) {
+  TopList t{0, 0};
   const int lane = lane_id();
+  int n = 0;
+  Key mine = 0;
+  for (int w = 0; w < waves; ++w) {
+    const int c = uniform(f.count[w]);
+    if (lane >= n && lane < n + c) mine = f.key[w][lane - n];
+    n += c;
+  }
   if (n > 64) {
-    for (int i = 0; i < n; i += 64)
-      top_offer(t, i + lane < n, i + lane < n ? f.value[i + lane] : 0.f, i + lane < n ? f.id[i + lane] : 0, top_k);
+    for (int w = 0; w < waves; ++w) top_offer(t, lane < f.count[w] ? f.key[w][lane] : 0, top_k);
     return t;
   }
-  const float v = lane < n ? f.value[lane] : -INFINITY;
-  const int id = lane < n ? f.id[lane] : kNoId;
+  f.all[lane] = mine;
+  __builtin_amdgcn_wave_barrier();
   int rank = 0;
-  for (int i = 0; i < n; ++i) rank += beats(lane_value(v, i), static_cast<int>(__builtin_amdgcn_readlane(id, i)), v, id);
+  for (int i = 0; i < n; i += 8) {   // beyond n the keys are 0 and beat nobody
+#pragma unroll
+    for (int j = 0; j < 8; ++j) rank += f.all[i + j] > mine;
+  }
   if (lane >= n) rank = lane;
   // every lane sends its element to the lane of its rank
-  t.value = __uint_as_float(__builtin_amdgcn_ds_permute(rank * 4, __float_as_uint(v)));
-  t.id = __builtin_amdgcn_ds_permute(rank * 4, id);
+  const uint32_t high = __builtin_amdgcn_ds_permute(rank * 4, static_cast<int>(mine >> 32));
+  const uint32_t low = __builtin_amdgcn_ds_permute(rank * 4, static_cast<int>(mine));
+  t.key = static_cast<Key>(high) << 32 | low;
   return t;
 }
 
@@ -248,17 +252,15 @@ __device__ __forceinline__ void finish_row(const LogprobForward &p, int row, Sof
     if (lane < p.top_k) {
       const int64_t at = static_cast<int64_t>(row) * p.top_k + lane;
       // a row of fewer than k numbers (the others NaN) has no more to name
-      const bool none = t.id == kNoId;
-      const float lp = none ? NAN : empty ? -INFINITY : fmaf(p.scale, t.value - a.m, -log_l);
+      const bool none = t.key == 0;
+      const float lp = none ? NAN : empty ? -INFINITY : fmaf(p.scale, value_of(t.key) - a.m, -log_l);
       for (int m = 0; m < p.members; ++m) {
-        if (p.top_ids) reinterpret_cast<int *>(p.top_ids + m * p.step)[at] = none ? -1 : t.id;
+        if (p.top_ids) reinterpret_cast<int *>(p.top_ids + m * p.step)[at] = none ? -1 : id_of(t.key);
         if (p.top_logprobs) reinterpret_cast<float *>(p.top_logprobs + m * p.step)[at] = lp;
       }
     }
   }
 }
-
-constexpr int kMaxWaves = 8, kMaxParts = 16;
 
 // Where a batch of a row lies: its first element, how many there are, and the first one's id.
 template <typename T>
@@ -294,7 +296,6 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
   const int row = uniform(static_cast<int>(blockIdx.x / p.parts)), part = uniform(static_cast<int>(blockIdx.x % p.parts));
   const float c2 = p.scale * kLog2e;
   const int64_t token = p.logprob ? p.tokens[row] : -1;
-  if (kTop && threadIdx.x == 0) found.count = 0;
   Softmax a{kLowest, 0.f, 0.f};
   const int64_t batches = static_cast<int64_t>(p.batches_per_member) * p.members;
   const int first = static_cast<int>(batches * part / p.parts), end = static_cast<int>(batches * (part + 1) / p.parts);
@@ -320,55 +321,56 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
   float of_token = 0.f;
   if (wave == 0 && token >= 0 && token < p.vocab) of_token = logit_of<T>(p, row, token);
   a = join_lanes(a, c2);
-  TopList t;
-  top_clear(t);
+  TopList t{0, 0};
   if (kTop || waves > 1) {
     if (lane == 0) sums[wave] = a;
     if constexpr (kTop) lane_best[wave][lane] = best;
     __syncthreads();
     if constexpr (kTop) {
       for (int w = 0; w < waves; ++w) best = fmaxf(best, lane_best[w][lane]);
-      const float bound = bound_of_lanes(best, p.top_k);
-      if (bound != -INFINITY) {
-        turn = at_note = 0;
-        for (int b = first + wave; b < end; b += waves) {
-          const bool near = notes[wave][at_note][lane] >= bound;
-          if (++turn == per_note) {
-            turn = 0;
-            ++at_note;
-          }
-          if (!__ballot(near) || *const_cast<volatile int *>(&found.count) > kMaxFound) continue;
-          const Batch<T> batch = batch_at<T>(p, row, b);
-          if (!near) continue;
-          u32x4 raw[kDeep];
-#pragma unroll
-          for (int k = 0; k < kDeep; ++k) {
-            const int c = (k * 64 + lane) * kRowVec<T>;
-            raw[k] = row_load<T, true>(batch.p + c, batch.left - c, sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u);
-          }
-#pragma unroll
-          for (int k = 0; k < kDeep; ++k)
-#pragma unroll
-            for (int e = 0; e < kRowVec<T>; ++e) {
-              const float x = row_get<T>(raw[k], e);
-              if (x >= bound) found_add(found, x, batch.id + (k * 64 + lane) * kRowVec<T> + e);
-            }
+      const uint32_t order = bound_of_lanes(order_of(best), p.top_k);
+      const bool bounded = order > kOrderOfMinusInf;
+      const float bound = value_of_order(order);
+      int n = bounded ? 0 : kRoom + 1;
+      turn = at_note = 0;
+      for (int b = first + wave; b < end && n <= kRoom; b += waves) {
+        const bool near = notes[wave][at_note][lane] >= bound;
+        if (++turn == per_note) {
+          turn = 0;
+          ++at_note;
         }
+        if (!__ballot(near)) continue;
+        const Batch<T> batch = batch_at<T>(p, row, b);
+        u32x4 raw[kDeep];
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k) {
+          const int c = (k * 64 + lane) * kRowVec<T>;
+          raw[k] = row_load<T, true>(batch.p + c, near ? batch.left - c : 0, kMinusInf<T>);
+        }
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k)
+#pragma unroll
+          for (int e = 0; e < kRowVec<T>; ++e) {
+            const float x = row_get<T>(raw[k], e);
+            found_add(found, wave, n, x >= bound, key_of(x, batch.id + (k * 64 + lane) * kRowVec<T> + e));
+          }
       }
+      if (lane == 0) found.count[wave] = n;
       __syncthreads();
       if (wave != 0) return;
-      if (bound != -INFINITY && found.count <= kMaxFound) {
-        t = found_best(found, uniform(found.count), p.top_k);
+      if (__ballot(lane < waves && found.count[lane % kMaxWaves] > kRoom) == 0) {
+        t = found_best(found, waves, p.top_k);
       } else {
         for (int b = first; b < end; ++b) {
           const int w = (b - first) % waves, i = (b - first) / waves;
-          const float noted = notes[w][i / per_note][lane];
           // ids grow from batch to batch: an equal value never beats a full list
-          if (!__ballot(noted > t.last_value || t.last_id == kNoId)) continue;
+          const uint32_t noted = order_of(notes[w][i / per_note][lane] + 0.f);
+          if (!__ballot(noted > static_cast<uint32_t>(t.last >> 32))) continue;
           const Batch<T> batch = batch_at<T>(p, row, b);
           for (int e = 0; e < kBatch<T> / 64; ++e) {
             const int c = e * 64 + lane;
-            top_offer(t, c < batch.left, element_at(batch, c), batch.id + c, p.top_k);
+            const float x = element_at(batch, c);
+            top_offer(t, c < batch.left && x == x ? key_of(x, batch.id + c) : 0, p.top_k);
           }
         }
       }
@@ -392,8 +394,7 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
   if (lane < 3) leave(mine + lane, lane == 0 ? a.m : lane == 1 ? a.l : a.w);
   if constexpr (kTop) {
     if (lane < p.top_k) {
-      leave(p.part_values + at * p.top_k + lane, t.value);
-      leave(p.part_ids + at * p.top_k + lane, t.id);
+      leave(p.part_keys + at * p.top_k + lane, t.key);
     }
   }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
@@ -411,44 +412,29 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
   if constexpr (kTop) {
     // the same bound over the parts' lists, all of them in registers
     constexpr int kHeld = kMaxParts * kMaxTop / 64;
-    const int64_t lists = static_cast<int64_t>(row) * p.parts * p.top_k;
+    uint64_t *lists = p.part_keys + static_cast<int64_t>(row) * p.parts * p.top_k;
     const int n = p.parts * p.top_k;
-    float v[kHeld];
-    int id[kHeld];
+    Key held[kHeld], most = 0;
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
-      const int i = k * 64 + lane;
-      v[k] = -INFINITY;
-      id[k] = kNoId;
-      if (i < n) {
-        v[k] = fetch(p.part_values + lists + i);
-        id[k] = fetch(p.part_ids + lists + i);
-      }
+      held[k] = 0;
+      if (k * 64 + lane < n) held[k] = fetch(lists + k * 64 + lane);
     }
-    best = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) best = fmaxf(best, v[k]);
-    const float bound = bound_of_lanes(best, p.top_k);
-    if (lane == 0) found.count = 0;
-    __builtin_amdgcn_wave_barrier();
-    if (bound != -INFINITY) {
+    for (int k = 0; k < kHeld; ++k) most = held[k] > most ? held[k] : most;
+    const uint32_t bound = bound_of_lanes(static_cast<uint32_t>(most >> 32), p.top_k);
+    int count = 0;
 #pragma unroll
-      for (int k = 0; k < kHeld; ++k)
-        if (v[k] >= bound) found_add(found, v[k], id[k]);
-    }
-    __builtin_amdgcn_wave_barrier();
-    const int all = uniform(*const_cast<volatile int *>(&found.count));
-    if (bound != -INFINITY && all <= kMaxFound) {
-      t = found_best(found, all, p.top_k);
+    for (int k = 0; k < kHeld; ++k)
+      found_add(found, 0, count, static_cast<uint32_t>(held[k] >> 32) >= bound && held[k] != 0, held[k]);
+    if (count <= kRoom) {
+      if (lane == 0) found.count[0] = count;
+      __builtin_amdgcn_wave_barrier();
+      t = found_best(found, 1, p.top_k);
     } else {
-      top_clear(t);
-#pragma unroll 1
-      for (int k = 0; k < kHeld; ++k) {
-        const int i = k * 64 + lane;
-        const float value = i < n ? fetch(p.part_values + lists + i) : -INFINITY;
-        const int name = i < n ? fetch(p.part_ids + lists + i) : kNoId;
-        top_offer(t, name != kNoId, value, name, p.top_k);
-      }
+      t = {0, 0};
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) top_offer(t, held[k], p.top_k);
     }
   }
   a = join_lanes(a, c2);
@@ -531,9 +517,8 @@ struct LogprobShape {
 
 template <typename A>
 bool shape_of(const A &a, const char *call, LogprobShape *out) {
-  const std::string who = std::string(call) + ": ";
   auto refuse = [&](const char *why) {
-    rsm::fail(who + why);
+    rsm::fail(std::string(call) + ": " + why);
     return false;
   };
   LogprobShape s;
@@ -676,8 +661,7 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
     const size_t n = a.rows * g.parts;
     char *work = moved(a.work, s.team.first);
     p.part_sums = reinterpret_cast<float4 *>(work);
-    p.part_values = reinterpret_cast<float *>(work + n * sizeof(float4));
-    p.part_ids = reinterpret_cast<int *>(p.part_values + n * a.top_k);
+    p.part_keys = reinterpret_cast<uint64_t *>(work + n * sizeof(float4));
     p.arrived = reinterpret_cast<unsigned *>(moved(a.pSync, s.team.first));
   }
   const dim3 grid(static_cast<unsigned>(a.rows * g.parts)), block(static_cast<unsigned>(g.waves * 64));

@@ -534,9 +534,8 @@ size_t type_size(int dtype) { return dtype == RSM_FLOAT ? 4 : dtype == RSM_BF16 
 // What a call's sizes and numbers come to, or false with the error set.  A = either argument struct.
 template <typename A>
 bool shape_of(const A &a, const char *call, size_t partial_ld, size_t normed_ld, rsm::Members *members, NormShape *out) {
-  const std::string who = std::string(call) + ": ";
   auto refuse = [&](const char *why) {
-    rsm::fail(who + why);
+    rsm::fail(std::string(call) + ": " + why);
     return false;
   };
   if (!type_size(a.dtype)) return refuse("dtype must be RSM_FLOAT or RSM_BF16");

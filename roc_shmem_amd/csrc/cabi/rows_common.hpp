@@ -3,7 +3,6 @@
 #define ROCSHMEM_MI355X_ROWS_COMMON_HPP
 
 #include <string>
-#include <vector>
 
 #include "cabi_common.hpp"
 
@@ -20,7 +19,8 @@ struct Members {
 };
 
 // The symmetric operands of one call: every one has to lie in a live allocation, and none that the
-// call writes may share bytes with another, unless the two are one array on purpose.
+// call writes may share bytes with another, unless the two are one array on purpose.  (A call of few
+// rows takes the GPU about as long as the host: no allocation and no text here but for a refusal.)
 class Operands {
  public:
   explicit Operands(const char *call) : call_(call) {}
@@ -30,20 +30,28 @@ class Operands {
     add(p, name, rows && cols ? ((rows - 1) * ld + cols) * size : 0, written);
   }
   void add(const void *p, const char *name, size_t bytes, bool written) {
-    if (p) spans_.push_back({static_cast<const char *>(p), bytes, name, written, nullptr});
+    if (p) spans_[count_++] = {static_cast<const char *>(p), bytes, name, written, nullptr};
   }
   // The operand added last may be the very array `p`: each row of `p` is read before it is written.
   void or_same_as(const void *p) {
-    if (!spans_.empty() && spans_.back().p == p) spans_.back().same = p;
+    if (count_ && spans_[count_ - 1].p == p) spans_[count_ - 1].same = p;
   }
 
   bool ok() const {
-    for (const Span &s : spans_) {
+    const auto *rt = rocshmem::host::Runtime::get();
+    for (int i = 0; i < count_; ++i) {
+      const Span &s = spans_[i];
+      const size_t offset = static_cast<size_t>(s.p - rt->arena());
+      if (s.p >= rt->arena() && offset < rt->slice_stride()) {
+        const size_t end = rt->allocation_end(offset);
+        if (end != rocshmem::host::Pow2Allocator::kNoOffset && s.bytes <= end - offset) continue;
+      }
       const std::string what = std::string(call_) + ": " + s.name;
-      if (!check_symmetric(s.p, what.c_str()) || !check_extent(s.p, s.bytes, what.c_str())) return false;
+      if (check_symmetric(s.p, what.c_str()) && check_extent(s.p, s.bytes, what.c_str())) fail(what + " is refused");
+      return false;
     }
-    for (size_t i = 0; i < spans_.size(); ++i)
-      for (size_t j = 0; j < i; ++j) {
+    for (int i = 0; i < count_; ++i)
+      for (int j = 0; j < i; ++j) {
         const Span &a = spans_[i], &b = spans_[j];
         if (!(a.written || b.written) || !(a.p < b.p + b.bytes && b.p < a.p + a.bytes)) continue;
         if (a.p == b.p && ((a.same == b.p && !b.written) || (b.same == a.p && !a.written))) continue;
@@ -61,8 +69,10 @@ class Operands {
     bool written;
     const void *same;
   };
+  static constexpr int kMost = 16;   // no call has more operands
   const char *call_;
-  std::vector<Span> spans_;
+  Span spans_[kMost];
+  int count_ = 0;
 };
 
 // False, with the error set, when `team` is none; otherwise its members.
