@@ -14,6 +14,7 @@
 // logits are all at the type's lowest value come out as any other row of equal logits.  A logit at
 // minus infinity has probability 0 and adds nothing to the entropy; m starts at the lowest finite
 // value, not at minus infinity, so that such logits never meet an infinite m.
+#include <cfloat>
 #include <cmath>
 
 #include "roc_shmem.hpp"
@@ -525,7 +526,7 @@ bool shape_of(const A &a, const char *call, LogprobShape *out) {
   if (!type_size(a.dtype)) return refuse("dtype must be RSM_FLOAT or RSM_BF16");
   if (a.vocab < 1 || a.vocab > 0x3fffffffull) return refuse("vocab must be in [1, 2^30)");
   if (a.rows >= 1u << 22) return refuse("rows must be below 2^22");
-  if (!(a.scale > 0.f) || !std::isfinite(a.scale)) return refuse("scale must be a positive number");
+  if (!(a.scale >= FLT_MIN) || !std::isfinite(a.scale * kLog2e)) return refuse("scale must be a positive (normal) number below 2^127");
   if (!rsm::members_of(a.team, call, &s.team)) return false;
   s.shard = a.shard ? a.shard : (a.vocab + s.team.size - 1) / s.team.size;
   if (s.shard > 0x3fffffffull || s.shard * s.team.size < a.vocab) return refuse("the members' shards do not cover the vocabulary");
@@ -551,12 +552,13 @@ LogprobPlan plan_of(const LogprobShape &s, int dtype, size_t rows, size_t vocab,
   g.batches = static_cast<int>((width_of(s, vocab) + batch - 1) / batch);
   const int64_t all = static_cast<int64_t>(g.batches) * s.team.size;
   g.parts = 1;
-  // Few rows: several workgroups to a row, so that the chip has some 512 to run, each with a batch for
-  // each of its waves.  More and smaller ones lose more in the joining than they win (one row of 128000
-  // bf16 with 20 alternatives: 8 workgroups of 8 waves 14.7 us, 16 of 4 15.3, 32 of 2 18.1, 64 of 1 24).
+  // Few rows: several workgroups to a row, so that the chip has some 512 to run, each with four batches
+  // at least, one for each of its waves: then a SIMD has one wave to run.  More and smaller ones lose more
+  // in the joining than they win (one row of 128000 bf16 with 20 alternatives: 8 workgroups of 8 waves
+  // 11.3 us, 16 of 4 10.9, 32 of 2 11.3; 64 x 50257 float with 5: 512 workgroups 11.6, 1024 12.2).
   if (rows && rows < 256) {
     int64_t parts = 512 / static_cast<int64_t>(rows);
-    const int64_t most = (all + kMaxWaves - 1) / kMaxWaves;
+    const int64_t most = (all + 3) / 4;
     if (parts > most) parts = most;
     if (parts > kMaxParts) parts = kMaxParts;
     g.parts = parts < 1 ? 1 : static_cast<int>(parts);
@@ -628,15 +630,15 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
   const size_t size = type_size(a.dtype);
   rsm::Operands o(call);
   o.matrix(a.logits, "logits", a.rows, width_of(s, a.vocab), s.ld, size, false);
-  o.add(a.tokens, "tokens", a.rows * 8, false);
-  o.add(a.logprob, "logprob", a.rows * 4, true);
-  o.add(a.entropy, "entropy", a.rows * 4, true);
-  o.add(a.lse, "lse", a.rows * 4, true);
-  o.add(a.top_ids, "top_ids", a.rows * a.top_k * 4, true);
-  o.add(a.top_logprobs, "top_logprobs", a.rows * a.top_k * 4, true);
+  o.add(a.tokens, "tokens", a.rows * 8, 8, false);
+  o.add(a.logprob, "logprob", a.rows * 4, 4, true);
+  o.add(a.entropy, "entropy", a.rows * 4, 4, true);
+  o.add(a.lse, "lse", a.rows * 4, 4, true);
+  o.add(a.top_ids, "top_ids", a.rows * a.top_k * 4, 4, true);
+  o.add(a.top_logprobs, "top_logprobs", a.rows * a.top_k * 4, 4, true);
   if (g.parts > 1) {
-    o.add(a.work, "work (rsm_logprob_work_bytes)", g.work_bytes, true);
-    o.add(a.pSync, "pSync (ROC_SHMEM_REDUCE_SYNC_SIZE longs)", ROC_SHMEM_REDUCE_SYNC_SIZE * sizeof(long), true);
+    o.add(a.work, "work (rsm_logprob_work_bytes)", g.work_bytes, 16, true);
+    o.add(a.pSync, "pSync (ROC_SHMEM_REDUCE_SYNC_SIZE longs)", ROC_SHMEM_REDUCE_SYNC_SIZE * sizeof(long), sizeof(long), true);
   }
   if (!o.ok()) return -1;
   LogprobForward p{};
@@ -692,12 +694,12 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   const size_t size = type_size(a.dtype);
   rsm::Operands o(call);
   o.matrix(a.logits, "logits", a.rows, width, s.ld, size, false);
-  o.add(a.tokens, "tokens", a.rows * 8, false);
-  o.add(a.lse, "lse", a.rows * 4, false);
-  o.add(a.entropy, "entropy", a.rows * 4, false);
-  o.add(a.grad_logprob, "grad_logprob", a.rows * 4, false);
-  o.add(a.grad_entropy, "grad_entropy", a.rows * 4, false);
-  o.add(a.grad_lse, "grad_lse", a.rows * 4, false);
+  o.add(a.tokens, "tokens", a.rows * 8, 8, false);
+  o.add(a.lse, "lse", a.rows * 4, 4, false);
+  o.add(a.entropy, "entropy", a.rows * 4, 4, false);
+  o.add(a.grad_logprob, "grad_logprob", a.rows * 4, 4, false);
+  o.add(a.grad_entropy, "grad_entropy", a.rows * 4, 4, false);
+  o.add(a.grad_lse, "grad_lse", a.rows * 4, 4, false);
   o.matrix(a.grad_logits, "grad_logits", a.rows, width, grad_ld, size, true);
   if (grad_ld == s.ld) o.or_same_as(a.logits);
   if (!o.ok()) return -1;

@@ -640,9 +640,9 @@ int rsm_norm_to_all(const rsm_norm_args_t *args, void *stream) {
   rsm::Operands o(call);
   o.matrix(a.source, "source", a.rows, a.cols, source_ld, size, false);
   o.matrix(a.residual, "residual", held, a.cols, ld, size, false);
-  o.add(a.pre_weight, "pre_weight", a.cols * size, false);
-  o.add(a.post_weight, "post_weight", a.cols * size, false);
-  o.add(a.gate, "gate", gate_rows(s) * a.cols * size, false);
+  o.add(a.pre_weight, "pre_weight", a.cols * size, size, false);
+  o.add(a.post_weight, "post_weight", a.cols * size, size, false);
+  o.add(a.gate, "gate", gate_rows(s) * a.cols * size, size, false);
   o.matrix(a.residual_out, "residual_out", held, a.cols, ld, size, true);
   o.or_same_as(a.residual);
   o.matrix(a.normed, "normed", a.rows, a.cols, normed_ld, size, true);
@@ -702,17 +702,17 @@ int rsm_norm_to_all_grad(const rsm_norm_grad_args_t *args, void *stream) {
   o.matrix(a.residual_out, "residual_out", mine, a.cols, ld, size, false);
   o.matrix(a.total, "total", shared, a.cols, a.cols, size, false);
   o.matrix(a.grad_residual_out, "grad_residual_out", mine, a.cols, ld, size, false);
-  o.add(a.pre_weight, "pre_weight", a.cols * size, false);
-  o.add(a.post_weight, "post_weight", a.cols * size, false);
-  o.add(a.gate, "gate", gate_rows(s) * a.cols * size, false);
+  o.add(a.pre_weight, "pre_weight", a.cols * size, size, false);
+  o.add(a.post_weight, "post_weight", a.cols * size, size, false);
+  o.add(a.gate, "gate", gate_rows(s) * a.cols * size, size, false);
   o.matrix(a.grad_source, "grad_source", a.rows, a.cols, source_ld, size, true);
   if (source_ld == normed_ld) o.or_same_as(a.grad_normed);
   o.matrix(a.grad_residual, "grad_residual", mine, a.cols, ld, size, true);
   o.or_same_as(a.grad_residual_out);
-  o.add(a.grad_pre_weight, "grad_pre_weight", a.cols * 4, true);
-  o.add(a.grad_post_weight, "grad_post_weight", a.cols * 4, true);
-  o.add(a.grad_gate, "grad_gate", gate_rows(s) * a.cols * 4, true);
-  if (sums) o.add(a.work, "work (rsm_norm_grad_work_bytes)", g.part_bytes * g.parts, true);
+  o.add(a.grad_pre_weight, "grad_pre_weight", a.cols * 4, 4, true);
+  o.add(a.grad_post_weight, "grad_post_weight", a.cols * 4, 4, true);
+  o.add(a.grad_gate, "grad_gate", gate_rows(s) * a.cols * 4, 4, true);
+  if (sums) o.add(a.work, "work (rsm_norm_grad_work_bytes)", g.part_bytes * g.parts, 16, true);
   if (!o.ok()) return -1;
   if (!a.grad_gate && !sums && a.rows == 0) return 0;
 

@@ -27,10 +27,11 @@ class Operands {
 
   // rows x cols elements of `size` bytes, `ld` elements from row to row.
   void matrix(const void *p, const char *name, size_t rows, size_t cols, size_t ld, size_t size, bool written) {
-    add(p, name, rows && cols ? ((rows - 1) * ld + cols) * size : 0, written);
+    add(p, name, rows && cols ? ((rows - 1) * ld + cols) * size : 0, size, written);
   }
-  void add(const void *p, const char *name, size_t bytes, bool written) {
-    if (p) spans_[count_++] = {static_cast<const char *>(p), bytes, name, written, nullptr};
+  // `bytes` bytes that begin at a multiple of `align`.
+  void add(const void *p, const char *name, size_t bytes, size_t align, bool written) {
+    if (p) spans_[count_++] = {static_cast<const char *>(p), bytes, align, name, written, nullptr};
   }
   // The operand added last may be the very array `p`: each row of `p` is read before it is written.
   void or_same_as(const void *p) {
@@ -44,10 +45,10 @@ class Operands {
       const size_t offset = static_cast<size_t>(s.p - rt->arena());
       if (s.p >= rt->arena() && offset < rt->slice_stride()) {
         const size_t end = rt->allocation_end(offset);
-        if (end != rocshmem::host::Pow2Allocator::kNoOffset && s.bytes <= end - offset) continue;
+        if (end != rocshmem::host::Pow2Allocator::kNoOffset && s.bytes <= end - offset && offset % s.align == 0) continue;
       }
       const std::string what = std::string(call_) + ": " + s.name;
-      if (check_symmetric(s.p, what.c_str()) && check_extent(s.p, s.bytes, what.c_str())) fail(what + " is refused");
+      if (check_symmetric(s.p, what.c_str()) && check_extent(s.p, s.bytes, what.c_str())) fail(what + " is not aligned to " + std::to_string(s.align) + " bytes");
       return false;
     }
     for (int i = 0; i < count_; ++i)
@@ -64,7 +65,7 @@ class Operands {
  private:
   struct Span {
     const char *p;
-    size_t bytes;
+    size_t bytes, align;
     const char *name;
     bool written;
     const void *same;

@@ -134,7 +134,7 @@ def run_forward(c, *, in_place=False, keep=True, normed=True, stream=None):
     return args
 
 
-def run_backward(c, *, in_place=False, has_normed=True, has_out=True, sums=True):
+def run_backward(c, *, in_place=False, has_normed=True, has_out=True, sums=True, without=()):
     partials = [c.numbers(c.rows, c.cols) for _ in range(c.size)]
     x, total, gout = (c.numbers(c.rows, c.cols, s) for s in (2.0, 1.5, 1.0))
     gn = c.rows_of(c.rows, c.cols, c.cols + c.pad) if has_normed else None
@@ -153,6 +153,8 @@ def run_backward(c, *, in_place=False, has_normed=True, has_out=True, sums=True)
             arrays["grad_post_weight"] = c.rows_of(1, c.cols, 0, np.float32)
         if c.gates:
             arrays["grad_gate"] = c.rows_of(c.gates, c.cols, 0, np.float32)
+    for n in without:
+        arrays.pop(n)
     results = [n for n in arrays if n in ("grad_source", "grad_residual", "grad_pre_weight", "grad_post_weight", "grad_gate")]
     for n in results:
         arrays[n].remember()
@@ -246,6 +248,51 @@ def test_optional_operands():
         run_backward(Case(rs.BF16, 12, 520, 4), has_normed=False)
         run_backward(Case(rs.FLOAT, 12, 520, 4, gate=3), sums=False)
         run_backward(Case(rs.FLOAT, 12, 520, 4, gate=0, post=False))
+        for without in (("grad_residual",), ("grad_pre_weight",), ("grad_post_weight", "grad_gate"), ("grad_pre_weight", "grad_post_weight")):
+            for gate in (1, 3):
+                run_backward(Case(rs.BF16, 12, 520, 4, gate=gate), without=without)
+
+
+def test_rows_beyond_4_gib():
+    """Strides that take the last rows past 2^32 bytes of their arrays' start."""
+    rows, cols, ld = 9, 600, 300_000_001
+    rs.roc_shmem_init(1, 64 << 30, 4, 1024)
+    try:
+        rng = np.random.default_rng(2)
+        numbers = lambda: ref.to_type(rs.BF16, rng.standard_normal((rows, cols)))  # noqa: E731
+        y, x = numbers(), numbers()
+
+        def far(values):
+            a = rs.sym_array((rows - 1) * ld + cols, np.uint16)
+            for r in range(rows if values is not None else 0):
+                a.write(0, values[r], r * ld)
+            return a
+
+        def near(a):
+            return np.stack([a.read(0, cols, r * ld) for r in range(rows)])
+
+        source, stream, total = far(y), far(x), rs.sym_array(rows * cols, np.uint16)
+        fields = dict(dtype=rs.BF16, flags=rs.NORM_POST, team=rs.roc_shmem_team_world(), rows=rows, cols=cols, eps=EPS,
+                      residual_scale=A, block_scale=B, source_ld=ld, residual_ld=ld, normed_ld=ld)
+        formula = dict(pre=None, post=None, gate=None, has_post=True, rows_per_gate=0, eps=float(np.float32(EPS)), a=A, b=B, o=O)
+        f = lambda v: ref.from_type(rs.BF16, v)  # noqa: E731
+        rs.roc_shmem_norm_to_all(rs.NormArgs(source=source, residual=stream, residual_out=stream, normed=source, total=total, **fields))
+        rs.synchronize()
+        want = ref.norm_forward(f(y)[None], f(x), **formula)
+        ref.check("normed", rs.BF16, near(source), *want["normed"])
+        ref.check("residual_out", rs.BF16, near(stream), *want["residual_out"])
+        out, kept, dn, dx = near(stream), total.read(0).reshape(rows, cols), numbers(), numbers()
+        for r in range(rows):
+            source.write(0, dn[r], r * ld)
+        grad = far(dx)
+        rs.roc_shmem_norm_to_all_grad(rs.NormGradArgs(grad_normed=source, grad_source=source, residual_out=stream, total=total,
+                                                      grad_residual_out=grad, grad_residual=grad, **fields))
+        rs.synchronize()
+        want = ref.norm_backward(f(dn)[None], f(dx), f(out), f(kept), **formula)
+        ref.check("grad_source", rs.BF16, near(source), *want["grad_source"])
+        ref.check("grad_residual", rs.BF16, near(grad), *want["grad_residual"])
+    finally:
+        rs.roc_shmem_finalize()
 
 
 @pytest.mark.parametrize("rows_per_gate", [1, 3, 4097, 5000])

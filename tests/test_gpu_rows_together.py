@@ -34,6 +34,7 @@ def test_operands_that_do_not_fit_or_overlap_are_refused():
                              (dict(source=rs.roc_shmem_ptr(source.addr, 1)), "symmetric"), (dict(team=12345), "team"),
                              (dict(normed=x), "overlap|fit"), (dict(residual_out=source), "overlap|fit"), (dict(total=out), "overlap"),
                              (dict(normed=source, source_ld=512 + 3), "overlap|fit"), (dict(normed=source.addr + 16), "overlap|fit"),
+                             (dict(source=source.addr + 2), "aligned|fit"), (dict(gate=source.addr + 1), "aligned"),
                              (dict(residual_out=c.weights and fields["pre_weight"].addr), "overlap|fit")]:
             refused(rs.roc_shmem_norm_to_all, rs.NormArgs(**{**fields, **change}), word)
         g = dict(c.fields, grad_normed=h, residual_out=x, total=c.shared(), grad_source=source, grad_residual=out,
@@ -41,13 +42,17 @@ def test_operands_that_do_not_fit_or_overlap_are_refused():
         refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(**g), "work")
         refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(work=small, **g), "work")
         refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(work=source, **g), "overlap|fit")
+        wide = rs.sym_array(1 << 22, np.uint8)
+        refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(work=wide.addr + 4, **g), "aligned")
         d = LogprobCase(rs.FLOAT, 8, 100000, 4, top_k=3)      # so few rows of so many share a workspace
         o = d.outputs()
         args = d.call(o)
         for change, word in [(dict(work=None), "work"), (dict(pSync=None), "pSync"), (dict(pSync=small), "pSync"),
                              (dict(logits_ld=1 << 22), "logits"), (dict(lse=o["entropy"]), "overlap"),
                              (dict(lse=d.array), "overlap|fit"), (dict(shard=200), "cover"), (dict(logits_ld=24999), "stride"),
-                             (dict(team=0), "team"), (dict(tokens=outside.addr), "symmetric")]:
+                             (dict(team=0), "team"), (dict(tokens=outside.addr), "symmetric"),
+                             (dict(tokens=d.token_array.addr + 4), "aligned"), (dict(pSync=wide.addr + 4), "aligned"),
+                             (dict(lse=wide.addr + 2), "aligned")]:
             fields = dict(top_k=3, work=args.work, pSync=args.pSync, **{**d.fields, **o})
             refused(rs.roc_shmem_logprob_to_all, rs.LogprobArgs(**{**fields, **change}), word)
         lse = d.numbers(np.zeros(8), np.float32)

@@ -16,7 +16,7 @@ REFUSED = [
     (rs.roc_shmem_norm_to_all, rs.NormArgs, NORM, [
         (dict(dtype=rs.DOUBLE), "dtype"), (dict(dtype=-1), "dtype"), (dict(flags=4), "flags"), (dict(cols=0), "cols"),
         (dict(cols=16385), "cols"), (dict(rows=1 << 22), "rows"), (dict(source_ld=7), "stride"), (dict(normed_ld=7), "stride"),
-        (dict(residual_ld=7), "stride"), (dict(source_ld=1 << 60), "stride"), (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"),
+        (dict(residual_ld=7), "stride"), (dict(source_ld=1 << 60), "stride"), (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"), (dict(eps=1e-40), "eps"),
         (dict(eps=float("nan")), "eps"), (dict(residual_scale=float("inf")), "finite"), (dict(block_scale=float("nan")), "finite"),
         (dict(weight_offset=float("inf")), "finite"), (dict(post_weight=128), "post_weight"), (dict(source=None), "source"),
         (dict(residual=None), "residual"), (dict(residual_out=None), "residual_out"),
@@ -30,6 +30,7 @@ REFUSED = [
     (rs.roc_shmem_logprob_to_all, rs.LogprobArgs, LOGPROB, [
         (dict(dtype=rs.LONG), "dtype"), (dict(vocab=0), "vocab"), (dict(vocab=1 << 30), "vocab"), (dict(rows=1 << 22), "rows"),
         (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+        (dict(scale=3e38), "scale"), (dict(scale=1e-40), "scale"),
         (dict(logits=None), "logits"), (dict(tokens=None), "tokens"), (dict(logprob=None), "no result"), (dict(top_k=3), "top_k"),
         (dict(top_ids=128), "top_k"), (dict(top_k=33, top_ids=128, vocab=100), "top_k"), (dict(top_k=9, top_ids=128), "top_k"),
         (dict(top_k=-1, top_ids=128), "top_k")]),
