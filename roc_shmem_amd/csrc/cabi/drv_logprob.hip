@@ -42,9 +42,12 @@ struct LogprobForward {
   const char *logits;
   const int64_t *tokens;
   char *logprob, *entropy, *lse, *top_ids, *top_logprobs;
-  // A row is cut into batches (kBatch elements, never across members); workgroup
-  // q of `parts` takes its share of them in order.
-  int batches_per_member, parts;
+  // A row is cut into batches of kBatch elements, 64 lanes x kDeep vectors, in ascending order of ids;
+  // workgroup q of `parts` takes its share of them in order.  Either every member's part is cut for
+  // itself (batches_per_member), or, where that would leave the last batches mostly empty (kPacked),
+  // the parts' vectors (vecs of them to a member) are numbered through and 256 of them make a batch.
+  int batches, batches_per_member, parts;
+  unsigned vecs, per_vecs;   // per_vecs: 2^32 / vecs, rounded up (exact for as few vectors); 0: vecs is 1
   float4 *part_sums;     // [rows][parts]: m, l, w
   uint64_t *part_keys;   // [rows][parts][top_k]
   unsigned *arrived;     // [rows], a 64-bit word apart, 0 on entry and on return
@@ -82,17 +85,61 @@ __device__ __forceinline__ Softmax join_lanes(Softmax a, float c2) {
 template <typename T>
 constexpr uint32_t kMinusInf = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 
-// One batch of a wave: `left` elements of the member's part from `p` on.  Returns the largest of this
-// lane's elements.
-template <typename T, bool kNt>
-__device__ __forceinline__ float take_batch(const T *p, int left, float c2, Softmax &a) {
+// Where a vector of a lane lies in a row: its first element, how many there are from it on (perhaps
+// none), and the first one's id.
+template <typename T>
+struct Place {
+  const T *p;
+  int left, id;
+};
+
+// Elements of member m's part from element `at` on.
+__device__ __forceinline__ int elements_left(const LogprobForward &p, int member, int at) {
+  const int64_t id = static_cast<int64_t>(member) * p.shard + at;
+  const int64_t rest = p.vocab - id;
+  if (rest <= 0) return 0;
+  return rest < p.shard - at ? static_cast<int>(rest) : p.shard - at;
+}
+
+// Vector `c / kRowVec` of batch b, with `c` the element's number within the batch.
+template <typename T, bool kPacked>
+struct Batch {
+  const LogprobForward &p;
+  int row, b;
+  const T *part;      // not packed: the batch's first element, and what is left from there on
+  int left, id;
+  __device__ __forceinline__ Batch(const LogprobForward &p_, int row_, int b_) : p(p_), row(row_), b(b_) {
+    if constexpr (!kPacked) {
+      const int member = uniform(b / p.batches_per_member);
+      const int at = (b - member * p.batches_per_member) * kBatch<T>;
+      left = elements_left(p, member, at);
+      id = static_cast<int>(static_cast<int64_t>(member) * p.shard + at);
+      part = reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at;
+    }
+  }
+  __device__ __forceinline__ Place<T> at(int c) const {
+    if constexpr (kPacked) {
+      const unsigned j = static_cast<unsigned>(b * kBatch<T> + c) / kRowVec<T>;
+      const int member = static_cast<int>(p.per_vecs ? __umulhi(j, p.per_vecs) : j);
+      const int off = static_cast<int>(j - member * p.vecs) * kRowVec<T> + c % kRowVec<T>;
+      const int rest = member < p.members ? elements_left(p, member, off) : 0;
+      return {reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + off, rest, member * p.shard + off};
+    } else {
+      return {part + c, left - c, id + c};
+    }
+  }
+};
+
+// One batch of a wave.  Returns the largest of this lane's elements.
+template <typename T, bool kNt, bool kPacked>
+__device__ __forceinline__ float take_batch(const Batch<T, kPacked> &batch, float c2, Softmax &a) {
   constexpr int V = kRowVec<T>;
   const int lane = lane_id();
   u32x4 raw[kDeep];
 #pragma unroll
   for (int k = 0; k < kDeep; ++k) {
-    const int c = (k * 64 + lane) * V;
-    raw[k] = row_load<T, true, kNt>(p + c, left - c, kMinusInf<T>);
+    const Place<T> v = batch.at((k * 64 + lane) * V);
+    raw[k] = row_load<T, true, kNt>(v.p, v.left, kMinusInf<T>);
   }
   float best = -INFINITY;
 #pragma unroll
@@ -117,9 +164,10 @@ __device__ __forceinline__ float take_batch(const T *p, int left, float c2, Soft
 // groups' maxima is a bound that at least k elements of the row reach, and few more: with 64 groups
 // and k = 20 some 24.  Only batches whose noted maximum reaches the bound are read again (from the
 // caches), their elements above it are gathered in LDS, and one wave ranks them.  The price per logit
-// is nothing but the maximum that the softmax needs anyway.  Rows of which a wave finds more than
-// kRoom elements (equal values, or fewer numbers than k) are gone through once more in ascending
-// order of ids, batch by batch, into a sorted list.
+// is nothing but the maximum that the softmax needs anyway.  Where fewer than k groups have a number
+// above minus infinity, all such numbers are gathered, and the lowest ids at minus infinity follow
+// them.  Rows of which a wave finds more than kRoom elements (many equal values) are gone through
+// once more in ascending order of ids, batch by batch, into a sorted list.
 //
 // An element is a 64-bit key: its value, ordered as an unsigned number, above its id counted down, so
 // that the larger of two keys is the larger value or, of equal ones, the lower id; 0 is no element.
@@ -175,49 +223,70 @@ __device__ __forceinline__ void top_offer(TopList &t, Key offered, int top_k) {
   }
 }
 
-// Elements gathered by waves: each has room of its own, in LDS.
-struct Found {
-  Key key[kMaxWaves][kRoom];
-  int count[kMaxWaves];
-  Key all[64];
+// What a workgroup's waves share, in LDS: `waves` of each array.
+struct Shared {
+  float (*notes)[kNotes][64];   // [wave][note][lane]: the largest element of a batch, or of several
+  float (*best)[64];            // [wave][lane]: the largest element of all
+  Key (*found)[kRoom];          // [wave]: the elements it gathered
+  Key *all;                     // [64]
+  Softmax *sums;                // [wave]
+  int *count;                   // [wave]: how many it gathered, kRoom + 1 or more: too many
 };
+__host__ __device__ constexpr size_t shared_bytes(int waves, bool top) {
+  return waves * (sizeof(Softmax) + (top ? (kNotes + 1) * 64 * sizeof(float) + kRoom * sizeof(Key) + sizeof(int) : 0)) +
+         (top ? 64 * sizeof(Key) : 0);
+}
+__device__ __forceinline__ Shared shared_of(char *base, int waves, bool top) {
+  Shared s{};
+  if (top) {
+    s.found = reinterpret_cast<Key(*)[kRoom]>(base);
+    s.all = reinterpret_cast<Key *>(s.found + waves);
+    s.notes = reinterpret_cast<float(*)[kNotes][64]>(s.all + 64);
+    s.best = reinterpret_cast<float(*)[64]>(s.notes + waves);
+    s.count = reinterpret_cast<int *>(s.best + waves);
+    base = reinterpret_cast<char *>(s.count + waves);
+  }
+  s.sums = reinterpret_cast<Softmax *>(base);
+  return s;
+}
 
 // Appends the lanes' elements (hit: there is one) to a wave's; `n` counts on beyond the room.
-__device__ __forceinline__ void found_add(Found &f, int wave, int &n, bool hit, Key key) {
+__device__ __forceinline__ void found_add(Key *found, int &n, bool hit, Key key) {
   const uint64_t mask = __ballot(hit);
   if (mask == 0) return;
   const int at = n + rank_in_mask(mask);
-  if (hit && at < kRoom) f.key[wave][at] = key;
+  if (hit && at < kRoom) found[at] = key;
   n += __popcll(mask);
 }
 
 // What `waves` waves found, at most kRoom each, sorted by one wave.
-__device__ __forceinline__ TopList found_best(Found &f, int waves, int top_k) {
+__device__ __forceinline__ TopList found_best(const Shared &s, int waves, int top_k) {
   TopList t{0, 0};
   const int lane = lane_id();
   int n = 0;
   Key mine = 0;
   for (int w = 0; w < waves; ++w) {
-    const int c = uniform(f.count[w]);
-    if (lane >= n && lane < n + c) mine = f.key[w][lane - n];
+    const int c = uniform(s.count[w]);
+    if (lane >= n && lane < n + c) mine = s.found[w][lane - n];
     n += c;
   }
   if (n > 64) {
-    for (int w = 0; w < waves; ++w) top_offer(t, lane < f.count[w] ? f.key[w][lane] : 0, top_k);
+    for (int w = 0; w < waves; ++w) top_offer(t, lane < s.count[w] ? s.found[w][lane] : 0, top_k);
     return t;
   }
-  f.all[lane] = mine;
+  s.all[lane] = mine;
   __builtin_amdgcn_wave_barrier();
   int rank = 0;
   for (int i = 0; i < n; i += 8) {   // beyond n the keys are 0 and beat nobody
 #pragma unroll
-    for (int j = 0; j < 8; ++j) rank += f.all[i + j] > mine;
+    for (int j = 0; j < 8; ++j) rank += s.all[i + j] > mine;
   }
   if (lane >= n) rank = lane;
   // every lane sends its element to the lane of its rank
   const uint32_t high = __builtin_amdgcn_ds_permute(rank * 4, static_cast<int>(mine >> 32));
   const uint32_t low = __builtin_amdgcn_ds_permute(rank * 4, static_cast<int>(mine));
   t.key = static_cast<Key>(high) << 32 | low;
+  t.last = lane_key(t.key, top_k - 1);
   return t;
 }
 
@@ -263,54 +332,36 @@ __device__ __forceinline__ void finish_row(const LogprobForward &p, int row, Sof
   }
 }
 
-// Where a batch of a row lies: its first element, how many there are, and the first one's id.
 template <typename T>
-struct Batch {
-  const T *p;
-  int left, id;
-};
-template <typename T>
-__device__ __forceinline__ Batch<T> batch_at(const LogprobForward &p, int row, int b) {
-  const int member = uniform(b / p.batches_per_member);
-  const int at = (b - member * p.batches_per_member) * kBatch<T>;
-  const int64_t id = static_cast<int64_t>(member) * p.shard + at;
-  int left = p.shard - at;
-  if (id + left > p.vocab) left = id < p.vocab ? static_cast<int>(p.vocab - id) : 0;
-  return {reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at, left, static_cast<int>(id)};
-}
-
-template <typename T>
-__device__ __forceinline__ float element_at(const Batch<T> &b, int c) {
-  if constexpr (sizeof(T) == 4) return c < b.left ? b.p[c] : -INFINITY;
-  else return c < b.left ? bf16_bits_to_float(reinterpret_cast<const uint16_t *>(b.p)[c]) : -INFINITY;
+__device__ __forceinline__ float element_at(const Place<T> &v) {
+  if (v.left <= 0) return -INFINITY;
+  if constexpr (sizeof(T) == 4) return *v.p;
+  else return bf16_bits_to_float(*reinterpret_cast<const uint16_t *>(v.p));
 }
 
 // 64 vector registers at most, so that a compute unit holds four workgroups: while some rank their
 // row's alternatives the others stream.
-template <typename T, bool kTop, bool kNt>
+template <typename T, bool kTop, bool kNt, bool kPacked>
 __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForward p) {
-  __shared__ Softmax sums[kMaxWaves];
-  __shared__ float lane_best[kTop ? kMaxWaves : 1][64];
-  __shared__ float notes[kTop ? kMaxWaves : 1][kNotes][64];
-  __shared__ Found found;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = lane_id(), wave = uniform(static_cast<int>(threadIdx.x / 64)), waves = blockDim.x / 64;
+  const Shared sh = shared_of(lds, waves, kTop);
   const int row = uniform(static_cast<int>(blockIdx.x / p.parts)), part = uniform(static_cast<int>(blockIdx.x % p.parts));
   const float c2 = p.scale * kLog2e;
   const int64_t token = p.logprob ? p.tokens[row] : -1;
   Softmax a{kLowest, 0.f, 0.f};
-  const int64_t batches = static_cast<int64_t>(p.batches_per_member) * p.members;
-  const int first = static_cast<int>(batches * part / p.parts), end = static_cast<int>(batches * (part + 1) / p.parts);
+  const int first = static_cast<int>(static_cast<int64_t>(p.batches) * part / p.parts);
+  const int end = static_cast<int>(static_cast<int64_t>(p.batches) * (part + 1) / p.parts);
   // batches of this wave that share a note
   const int per_note = ((end - first + waves - 1) / waves + kNotes - 1) / kNotes;
   float best = -INFINITY, note = -INFINITY;
   int turn = 0, at_note = 0;
   for (int b = first + wave; b < end; b += waves) {
-    const Batch<T> batch = batch_at<T>(p, row, b);
-    const float here = take_batch<T, kNt>(batch.p, batch.left, c2, a);
+    const float here = take_batch<T, kNt>(Batch<T, kPacked>(p, row, b), c2, a);
     if constexpr (kTop) {
       best = fmaxf(best, here);
       note = fmaxf(note, here);
-      notes[wave][at_note][lane] = note;
+      sh.notes[wave][at_note][lane] = note;
       if (++turn == per_note) {
         turn = 0;
         ++at_note;
@@ -324,60 +375,63 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
   a = join_lanes(a, c2);
   TopList t{0, 0};
   if (kTop || waves > 1) {
-    if (lane == 0) sums[wave] = a;
-    if constexpr (kTop) lane_best[wave][lane] = best;
+    if (lane == 0) sh.sums[wave] = a;
+    if constexpr (kTop) sh.best[wave][lane] = best;
     __syncthreads();
     if constexpr (kTop) {
-      for (int w = 0; w < waves; ++w) best = fmaxf(best, lane_best[w][lane]);
+      for (int w = 0; w < waves; ++w) best = fmaxf(best, sh.best[w][lane]);
       const uint32_t order = bound_of_lanes(order_of(best), p.top_k);
       const bool bounded = order > kOrderOfMinusInf;
-      const float bound = value_of_order(order);
-      int n = bounded ? 0 : kRoom + 1;
+      const float bound = bounded ? value_of_order(order) : kLowest;
+      int n = 0;
       turn = at_note = 0;
       for (int b = first + wave; b < end && n <= kRoom; b += waves) {
-        const bool near = notes[wave][at_note][lane] >= bound;
+        const bool near = sh.notes[wave][at_note][lane] >= bound;
         if (++turn == per_note) {
           turn = 0;
           ++at_note;
         }
         if (!__ballot(near)) continue;
-        const Batch<T> batch = batch_at<T>(p, row, b);
+        const Batch<T, kPacked> batch(p, row, b);
         u32x4 raw[kDeep];
+        int id[kDeep];
 #pragma unroll
         for (int k = 0; k < kDeep; ++k) {
-          const int c = (k * 64 + lane) * kRowVec<T>;
-          raw[k] = row_load<T, true>(batch.p + c, near ? batch.left - c : 0, kMinusInf<T>);
+          const Place<T> v = batch.at((k * 64 + lane) * kRowVec<T>);
+          id[k] = v.id;
+          raw[k] = row_load<T, true>(v.p, near ? v.left : 0, kMinusInf<T>);
         }
 #pragma unroll
         for (int k = 0; k < kDeep; ++k)
 #pragma unroll
           for (int e = 0; e < kRowVec<T>; ++e) {
             const float x = row_get<T>(raw[k], e);
-            found_add(found, wave, n, x >= bound, key_of(x, batch.id + (k * 64 + lane) * kRowVec<T> + e));
+            found_add(sh.found[wave], n, x >= bound, key_of(x, id[k] + e));
           }
       }
-      if (lane == 0) found.count[wave] = n;
+      if (lane == 0) sh.count[wave] = n;
       __syncthreads();
       if (wave != 0) return;
-      if (__ballot(lane < waves && found.count[lane % kMaxWaves] > kRoom) == 0) {
-        t = found_best(found, waves, p.top_k);
-      } else {
-        for (int b = first; b < end; ++b) {
+      const bool room = __ballot(lane < waves && sh.count[lane % waves] > kRoom) == 0;
+      if (room) t = found_best(sh, waves, p.top_k);
+      if (!room || t.last == 0) {
+        // Ids grow from batch to batch: an equal value never beats a full list.  Behind all numbers
+        // above minus infinity (room) only elements at minus infinity are missing.
+        for (int b = first; b < end && !(room && t.last != 0); ++b) {
           const int w = (b - first) % waves, i = (b - first) / waves;
-          // ids grow from batch to batch: an equal value never beats a full list
-          const uint32_t noted = order_of(notes[w][i / per_note][lane] + 0.f);
+          const uint32_t noted = order_of(sh.notes[w][i / per_note][lane] + 0.f);
           if (!__ballot(noted > static_cast<uint32_t>(t.last >> 32))) continue;
-          const Batch<T> batch = batch_at<T>(p, row, b);
+          const Batch<T, kPacked> batch(p, row, b);
           for (int e = 0; e < kBatch<T> / 64; ++e) {
-            const int c = e * 64 + lane;
-            const float x = element_at(batch, c);
-            top_offer(t, c < batch.left && x == x ? key_of(x, batch.id + c) : 0, p.top_k);
+            const Place<T> v = batch.at(e * 64 + lane);
+            const float x = element_at(v);
+            top_offer(t, v.left > 0 && (room ? x == -INFINITY : x == x) ? key_of(x, v.id) : 0, p.top_k);
           }
         }
       }
     }
     if (wave != 0) return;
-    a = lane < waves ? sums[lane] : Softmax{kLowest, 0.f, 0.f};
+    a = lane < waves ? sh.sums[lane] : Softmax{kLowest, 0.f, 0.f};
     a = join_lanes(a, c2);
   }
   if (p.parts == 1) {
@@ -427,11 +481,11 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
     int count = 0;
 #pragma unroll
     for (int k = 0; k < kHeld; ++k)
-      found_add(found, 0, count, static_cast<uint32_t>(held[k] >> 32) >= bound && held[k] != 0, held[k]);
+      found_add(sh.found[0], count, static_cast<uint32_t>(held[k] >> 32) >= bound && held[k] != 0, held[k]);
     if (count <= kRoom) {
-      if (lane == 0) found.count[0] = count;
+      if (lane == 0) sh.count[0] = count;
       __builtin_amdgcn_wave_barrier();
-      t = found_best(found, 1, p.top_k);
+      t = found_best(sh, 1, p.top_k);
     } else {
       t = {0, 0};
 #pragma unroll
@@ -542,15 +596,25 @@ size_t width_of(const LogprobShape &s, size_t vocab) { return s.shard < vocab ? 
 
 // How a row is cut: batches per member, workgroups per row and waves per workgroup.
 struct LogprobPlan {
-  int batches, parts, waves;
+  int batches, batches_per_member, parts, waves;
+  unsigned vecs;
+  bool packed;
   size_t work_bytes;
 };
 
 LogprobPlan plan_of(const LogprobShape &s, int dtype, size_t rows, size_t vocab, int top_k) {
   LogprobPlan g{};
-  const int batch = dtype == RSM_BF16 ? kBatch<__hip_bfloat16> : kBatch<float>;
-  g.batches = static_cast<int>((width_of(s, vocab) + batch - 1) / batch);
-  const int64_t all = static_cast<int64_t>(g.batches) * s.team.size;
+  const int vec = dtype == RSM_BF16 ? kRowVec<__hip_bfloat16> : kRowVec<float>, batch_vecs = 64 * kDeep;
+  const size_t width = width_of(s, vocab);
+  g.vecs = static_cast<unsigned>((width + vec - 1) / vec);
+  g.batches_per_member = static_cast<int>((g.vecs + batch_vecs - 1) / batch_vecs);
+  // Numbering the vectors through costs some instructions per vector; it pays where cutting every
+  // member's part for itself would leave more than a seventh of the lanes idle.
+  g.packed = static_cast<size_t>(g.batches_per_member) * batch_vecs * 7 > static_cast<size_t>(g.vecs) * 8;
+  const int members = static_cast<int>((vocab + width - 1) / width) < s.team.size ? static_cast<int>((vocab + width - 1) / width) : s.team.size;
+  const int64_t all = g.packed ? (static_cast<int64_t>(members) * g.vecs + batch_vecs - 1) / batch_vecs
+                               : static_cast<int64_t>(members) * g.batches_per_member;
+  g.batches = static_cast<int>(all);
   g.parts = 1;
   // Few rows: several workgroups to a row, so that the chip has some 512 to run, each with four batches
   // at least, one for each of its waves: then a SIMD has one wave to run.  More and smaller ones lose more
@@ -576,14 +640,22 @@ const T *moved_as(const void *p, int64_t bytes) {
   return reinterpret_cast<const T *>(moved(p, bytes));
 }
 
+template <typename T, bool kTop, bool kNt>
+void launch_forward(const LogprobForward &p, bool packed, dim3 grid, int waves, hipStream_t st) {
+  const dim3 block(static_cast<unsigned>(waves * 64));
+  const size_t lds = shared_bytes(waves, kTop);
+  if (packed) hipLaunchKernelGGL((logprob_kernel<T, kTop, kNt, true>), grid, block, lds, st, p);
+  else hipLaunchKernelGGL((logprob_kernel<T, kTop, kNt, false>), grid, block, lds, st, p);
+}
+
 template <typename T>
-void launch_forward(const LogprobForward &p, dim3 grid, dim3 block, hipStream_t st, bool once) {
+void launch_forward(const LogprobForward &p, const LogprobPlan &g, dim3 grid, hipStream_t st, bool once) {
   if (p.top_k) {
-    if (once) hipLaunchKernelGGL((logprob_kernel<T, true, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((logprob_kernel<T, true, false>), grid, block, 0, st, p);
+    if (once) launch_forward<T, true, true>(p, g.packed, grid, g.waves, st);
+    else launch_forward<T, true, false>(p, g.packed, grid, g.waves, st);
   } else {
-    if (once) hipLaunchKernelGGL((logprob_kernel<T, false, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((logprob_kernel<T, false, false>), grid, block, 0, st, p);
+    if (once) launch_forward<T, false, true>(p, g.packed, grid, g.waves, st);
+    else launch_forward<T, false, false>(p, g.packed, grid, g.waves, st);
   }
 }
 
@@ -657,7 +729,10 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
   p.lse = moved(a.lse, s.team.first);
   p.top_ids = moved(a.top_ids, s.team.first);
   p.top_logprobs = moved(a.top_logprobs, s.team.first);
-  p.batches_per_member = g.batches;
+  p.batches = g.batches;
+  p.batches_per_member = g.batches_per_member;
+  p.vecs = g.vecs;
+  p.per_vecs = g.vecs > 1 ? static_cast<unsigned>(((uint64_t{1} << 32) + g.vecs - 1) / g.vecs) : 0;
   p.parts = g.parts;
   if (g.parts > 1) {
     const size_t n = a.rows * g.parts;
@@ -666,13 +741,13 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
     p.part_keys = reinterpret_cast<uint64_t *>(work + n * sizeof(float4));
     p.arrived = reinterpret_cast<unsigned *>(moved(a.pSync, s.team.first));
   }
-  const dim3 grid(static_cast<unsigned>(a.rows * g.parts)), block(static_cast<unsigned>(g.waves * 64));
+  const dim3 grid(static_cast<unsigned>(a.rows * g.parts));
   hipStream_t st = static_cast<hipStream_t>(stream);
   // Logits that the Infinity Cache could not hold anyway are read past it: 4096 x 131072 bf16 without
   // alternatives 168 us against 186; smaller ones may still lie there from the product that made them.
   const bool once = a.rows * a.vocab * size > rsm::kInfinityCacheBytes;
-  if (a.dtype == RSM_BF16) launch_forward<__hip_bfloat16>(p, grid, block, st, once);
-  else launch_forward<float>(p, grid, block, st, once);
+  if (a.dtype == RSM_BF16) launch_forward<__hip_bfloat16>(p, g, grid, st, once);
+  else launch_forward<float>(p, g, grid, st, once);
   return rsm::after_launch(call);
 }
 
