@@ -504,7 +504,10 @@ struct LogprobBackward {
   const int64_t *tokens;
   const float *lse, *entropy, *grad_logprob, *grad_entropy, *grad_lse;
   char *grad_logits;
-  int chunks;   // workgroups per row of a member
+  // A line is one member's part of a row.  Either `chunks` workgroups take a line, or, where that would
+  // leave them mostly idle (kPacked), the lines' vectors (vecs of them to a line) are numbered through.
+  int chunks;
+  unsigned vecs, per_vecs, per_members;   // per_*: 2^32 / *, rounded up (exact for what is divided); 0: * is 1
 };
 
 // Bound by memory: without its arithmetic the kernel takes as long (4096 x 131072 bf16, by process 354
@@ -514,50 +517,108 @@ constexpr int kGradLanes = 256, kGradDeep = 8;
 template <typename T>
 constexpr int kGradChunk = kGradLanes * kRowVec<T> * kGradDeep;
 
-template <typename T, bool kNt>
+// What the gradient of a row's logits depends on.
+struct RowGrads {
+  float lse, of_token, of_entropy, flat;
+  int64_t token;
+};
+__device__ __forceinline__ RowGrads row_grads(const LogprobBackward &p, int row) {
+  RowGrads r;
+  // A row without any logit above minus infinity has no probabilities: 0 throughout, as against an
+  // infinite normaliser.
+  r.lse = p.lse[row];
+  if (r.lse == -INFINITY) r.lse = INFINITY;
+  r.token = p.tokens ? p.tokens[row] : -1;
+  r.of_token = p.grad_logprob && r.token >= 0 && r.token < p.vocab ? p.scale * p.grad_logprob[row] : 0.f;
+  r.of_entropy = p.grad_entropy ? p.scale * p.grad_entropy[row] : 0.f;
+  r.flat = (p.grad_lse ? p.scale * p.grad_lse[row] : 0.f) - r.of_token - (p.grad_entropy ? r.of_entropy * p.entropy[row] : 0.f);
+  return r;
+}
+
+// The gradient of a vector of logits whose first element has id `id`.
+template <typename T>
+__device__ __forceinline__ u32x4 grad_of(const LogprobBackward &p, const RowGrads &r, u32x4 raw, int64_t id) {
+  const int64_t hit = r.token - id;
+  float d[kRowVec<T>];
+#pragma unroll
+  for (int e = 0; e < kRowVec<T>; ++e) {
+    const float lp = fmaf(row_get<T>(raw, e), p.scale, -r.lse);
+    d[e] = exp2_of(lp * kLog2e) * fmaf(-r.of_entropy, fmaxf(lp, kFarBelow), r.flat);
+    if (e == hit) d[e] += r.of_token;
+  }
+  return row_pack<T>(d);
+}
+
+// j / n for the small j of packed vectors and members; per_n: see LogprobBackward.
+__device__ __forceinline__ int divided(unsigned j, unsigned per_n) { return static_cast<int>(per_n ? __umulhi(j, per_n) : j); }
+
+template <typename T, bool kNt, bool kPacked>
 __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(LogprobBackward p) {
   constexpr int V = kRowVec<T>;
   const uint64_t b = static_cast<uint64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
-  const int chunk = uniform(static_cast<int>(b % p.chunks));
-  const int64_t line = uniform(static_cast<unsigned long>(b / p.chunks));
-  const int row = static_cast<int>(line / p.members), member = static_cast<int>(line % p.members);
-  if (row >= p.rows) return;
-  const int at = chunk * kGradChunk<T>;
-  const int64_t id = static_cast<int64_t>(member) * p.shard + at;
-  int left = p.shard - at;
-  if (id + left > p.vocab) left = id < p.vocab ? static_cast<int>(p.vocab - id) : 0;
-  if (left <= 0) return;
-  const T *x = reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at;
-  T *out = reinterpret_cast<T *>(p.grad_logits + member * p.step) + row * p.grad_ld + at;
   const int lane = threadIdx.x;
   u32x4 raw[kGradDeep];
+  if constexpr (kPacked) {
+    const uint64_t first = b * (kGradLanes * kGradDeep);
+    const uint64_t line0 = uniform(static_cast<unsigned long>(first / p.vecs));
+    const unsigned into = uniform(static_cast<uint32_t>(first % p.vecs));
+    const int64_t row0 = uniform(static_cast<unsigned long>(line0 / p.members));
+    const unsigned member0 = uniform(static_cast<uint32_t>(line0 % p.members));
+    auto at = [&](int k, int64_t *row, int *off, int *member) {
+      const unsigned j = into + k * kGradLanes + lane;
+      const int line = divided(j, p.per_vecs);
+      *off = static_cast<int>(j - line * p.vecs) * V;
+      const unsigned q = member0 + line;
+      const int down = divided(q, p.per_members);
+      *member = static_cast<int>(q) - down * p.members;
+      *row = row0 + down;
+      const int64_t left = p.vocab - (static_cast<int64_t>(*member) * p.shard + *off);
+      const int width = p.shard - *off;
+      return *row >= p.rows || left <= 0 ? 0 : left < width ? static_cast<int>(left) : width;
+    };
+    int64_t row;
+    int off, member;
 #pragma unroll
-  for (int k = 0; k < kGradDeep; ++k) {
-    const int c = (k * kGradLanes + lane) * V;
-    raw[k] = row_load<T, true>(x + c, left - c);
-  }
-  // A row without any logit above minus infinity has no probabilities: 0 throughout, as against an
-  // infinite normaliser.
-  float lse = p.lse[row];
-  if (lse == -INFINITY) lse = INFINITY;
-  const int64_t token = p.tokens ? p.tokens[row] : -1;
-  if (token >= p.vocab && chunk == 0 && member == 0 && lane == 0) status_raise(kStatusBadArgument);
-  const float of_token = p.grad_logprob && token >= 0 && token < p.vocab ? p.scale * p.grad_logprob[row] : 0.f;
-  const float of_entropy = p.grad_entropy ? p.scale * p.grad_entropy[row] : 0.f;
-  const float of_lse = p.grad_lse ? p.scale * p.grad_lse[row] : 0.f;
-  const float flat = of_lse - of_token - (p.grad_entropy ? of_entropy * p.entropy[row] : 0.f);
-  const int64_t hit = token - id;
-#pragma unroll
-  for (int k = 0; k < kGradDeep; ++k) {
-    const int c = (k * kGradLanes + lane) * V;
-    float d[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float lp = fmaf(row_get<T>(raw[k], e), p.scale, -lse);
-      d[e] = exp2_of(lp * kLog2e) * fmaf(-of_entropy, fmaxf(lp, kFarBelow), flat);
-      if (c + e == hit) d[e] += of_token;
+    for (int k = 0; k < kGradDeep; ++k) {
+      const int left = at(k, &row, &off, &member);
+      raw[k] = row_load<T, true>(reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + off, left);
     }
-    row_store<T, true, kNt>(out + c, left - c, row_pack<T>(d));
+#pragma unroll
+    for (int k = 0; k < kGradDeep; ++k) {
+      const int left = at(k, &row, &off, &member);
+      if (left > 0) {
+        const RowGrads r = row_grads(p, static_cast<int>(row));
+        if (r.token >= p.vocab && member == 0 && off == 0) status_raise(kStatusBadArgument);
+        row_store<T, true, kNt>(reinterpret_cast<T *>(p.grad_logits + member * p.step) + row * p.grad_ld + off, left,
+                                grad_of<T>(p, r, raw[k], static_cast<int64_t>(member) * p.shard + off));
+      }
+    }
+  } else {
+    const int chunk = uniform(static_cast<int>(b % p.chunks));
+    const int64_t line = uniform(static_cast<unsigned long>(b / p.chunks));
+    const int row = static_cast<int>(line / p.members), member = static_cast<int>(line % p.members);
+    if (row >= p.rows) return;
+    const int at = chunk * kGradChunk<T>;
+    const int64_t id = static_cast<int64_t>(member) * p.shard + at;
+    const int64_t rest = p.vocab - id;
+    const int left = rest <= 0 ? 0 : rest < p.shard - at ? static_cast<int>(rest) : p.shard - at;
+    const T *x = reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at;
+    T *out = reinterpret_cast<T *>(p.grad_logits + member * p.step) + row * p.grad_ld + at;
+    // a wave whose vectors lie behind the line's end has nothing to do
+    const int wave0 = uniform(lane & ~63);
+#pragma unroll
+    for (int k = 0; k < kGradDeep; ++k) {
+      const int c = (k * kGradLanes + lane) * V;
+      raw[k] = row_load<T, true>(x + c, left - c);
+    }
+    const RowGrads r = row_grads(p, row);
+    if (r.token >= p.vocab && chunk == 0 && member == 0 && lane == 0) status_raise(kStatusBadArgument);
+#pragma unroll
+    for (int k = 0; k < kGradDeep; ++k) {
+      const int c = (k * kGradLanes + lane) * V;
+      if ((k * kGradLanes + wave0) * V >= left) break;
+      row_store<T, true, kNt>(out + c, left - c, grad_of<T>(p, r, raw[k], id + c));
+    }
   }
 }
 
@@ -660,10 +721,19 @@ void launch_forward(const LogprobForward &p, const LogprobPlan &g, dim3 grid, hi
 }
 
 template <typename T>
-void launch_backward(const LogprobBackward &p, dim3 grid, hipStream_t st, bool large) {
-  if (large) hipLaunchKernelGGL((logprob_grad_kernel<T, true>), grid, dim3(kGradLanes), 0, st, p);
-  else hipLaunchKernelGGL((logprob_grad_kernel<T, false>), grid, dim3(kGradLanes), 0, st, p);
+void launch_backward(const LogprobBackward &p, dim3 grid, hipStream_t st, bool large, bool packed) {
+  const dim3 block(kGradLanes);
+  if (packed) {
+    if (large) hipLaunchKernelGGL((logprob_grad_kernel<T, true, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((logprob_grad_kernel<T, false, true>), grid, block, 0, st, p);
+  } else {
+    if (large) hipLaunchKernelGGL((logprob_grad_kernel<T, true, false>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((logprob_grad_kernel<T, false, false>), grid, block, 0, st, p);
+  }
 }
+
+// 2^32 / n rounded up, 0 for 1.
+unsigned per(unsigned n) { return n > 1 ? static_cast<unsigned>(((uint64_t{1} << 32) + n - 1) / n) : 0; }
 
 bool top_in_range(const char *call, int top_k, size_t vocab) {
   if (top_k >= 0 && top_k <= kMaxTop && static_cast<size_t>(top_k) <= vocab) return true;
@@ -732,7 +802,7 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
   p.batches = g.batches;
   p.batches_per_member = g.batches_per_member;
   p.vecs = g.vecs;
-  p.per_vecs = g.vecs > 1 ? static_cast<unsigned>(((uint64_t{1} << 32) + g.vecs - 1) / g.vecs) : 0;
+  p.per_vecs = per(g.vecs);
   p.parts = g.parts;
   if (g.parts > 1) {
     const size_t n = a.rows * g.parts;
@@ -795,16 +865,24 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   p.grad_entropy = moved_as<float>(a.grad_entropy, s.team.first);
   p.grad_lse = moved_as<float>(a.grad_lse, s.team.first);
   p.grad_logits = moved(a.grad_logits, s.team.first);
-  const size_t per = a.dtype == RSM_BF16 ? kGradChunk<__hip_bfloat16> : kGradChunk<float>;
-  p.chunks = static_cast<int>((width + per - 1) / per);
-  const size_t wgs = a.rows * p.members * static_cast<size_t>(p.chunks);
+  const size_t vec = a.dtype == RSM_BF16 ? kRowVec<__hip_bfloat16> : kRowVec<float>, most = kGradLanes * kGradDeep;
+  p.vecs = static_cast<unsigned>((width + vec - 1) / vec);
+  p.chunks = static_cast<int>((p.vecs + most - 1) / most);
+  p.per_vecs = per(p.vecs);
+  p.per_members = per(static_cast<unsigned>(p.members));
+  // Short lines would leave a workgroup without enough to do for its start: 4096 x 1000 bf16 over 8 members
+  // 173 us by lines and 16 numbered through.  Longer ones pay more for numbering (a row's numbers are
+  // read for every vector) than for waves that have nothing to do.
+  const bool packed = p.vecs < 512;
+  const size_t lines = a.rows * p.members;
+  const size_t wgs = packed ? (lines * p.vecs + most - 1) / most : lines * static_cast<size_t>(p.chunks);
   const size_t x = wgs < 0x800000 ? wgs : 0x800000, y = (wgs + x - 1) / x;
   if (y > 65535) return rsm::fail("logprob_to_all_grad: too many rows for one launch");
   const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(y));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool large = 2 * a.rows * a.vocab * size > rsm::kInfinityCacheBytes;
-  if (a.dtype == RSM_BF16) launch_backward<__hip_bfloat16>(p, grid, st, large);
-  else launch_backward<float>(p, grid, st, large);
+  if (a.dtype == RSM_BF16) launch_backward<__hip_bfloat16>(p, grid, st, large, packed);
+  else launch_backward<float>(p, grid, st, large, packed);
   return rsm::after_launch(call);
 }
 

@@ -67,10 +67,31 @@ __device__ __forceinline__ T *row_at(char *base, int64_t bytes, int64_t row, int
   return reinterpret_cast<T *>(base + bytes) + row * ld + col;
 }
 
+// How a row ends (kEnd).  kWhole: with a whole vector.  kShifted: inside one; the lane that holds the end
+// moves back to the row's last whole vector and makes some elements that its neighbour makes too, to
+// the same bits - rows are loaded, and stored, without a question - and leaves them out of sums over
+// the row.  kNarrow: rows shorter than a vector, element by element.
+enum RowEnd { kWhole = 0, kShifted = 1, kNarrow = 2 };
+
+// First column of a lane's vector v, kept inside the row.
+template <typename T, int kLanes, int kEnd>
+__device__ __forceinline__ int column(int cols, int lane, int v) {
+  const int c = (v * kLanes + lane) * kRowVec<T>;
+  return kEnd == kShifted && c < cols && c > cols - kRowVec<T> ? cols - kRowVec<T> : c;
+}
+// What a lane's element e of vector v counts in a sum over the row: its value, or 0 where the
+// neighbour counts it.
+template <typename T, int kLanes, int kEnd>
+__device__ __forceinline__ float counted(int cols, int lane, int v, int e, float value) {
+  if constexpr (kEnd != kShifted) return value;
+  const int c = (v * kLanes + lane) * kRowVec<T>;
+  return column<T, kLanes, kEnd>(cols, lane, v) + e >= c ? value : 0.f;
+}
+
 constexpr int kFoldDepth = 8;   // vectors of a lane, of several members, whose loads are in flight together
 
 // Sum over the members of one row's elements that this lane holds.
-template <typename T, int kLanes, int NV, bool kTail, bool kNt, int kAtOnce = kFoldDepth>
+template <typename T, int kLanes, int NV, int kEnd, bool kNt, int kAtOnce = kFoldDepth>
 __device__ __forceinline__ void fold_members(const NormShape &s, int members, const char *base, int64_t row, int64_t ld,
                                              int lane, float (&acc)[NV][kRowVec<T>]) {
   constexpr int V = kRowVec<T>;
@@ -85,9 +106,9 @@ __device__ __forceinline__ void fold_members(const NormShape &s, int members, co
     for (int k = 0; k < kDepth; ++k) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * kLanes + lane) * V;
+        const int c = column<T, kLanes, kEnd>(s.cols, lane, v);
         raw[k][v] = u32x4{0u, 0u, 0u, 0u};
-        if (m + k < members) raw[k][v] = row_load<T, kTail, kNt>(row_at<T>(base, (m + k) * s.step, row, ld, c), s.cols - c);
+        if (m + k < members) raw[k][v] = row_load<T, kEnd == kNarrow, kNt>(row_at<T>(base, (m + k) * s.step, row, ld, c), s.cols - c);
       }
     }
 #pragma unroll
@@ -99,12 +120,12 @@ __device__ __forceinline__ void fold_members(const NormShape &s, int members, co
   }
 }
 
-template <typename T, int kLanes, int NV, bool kTail, bool kNt = false>
+template <typename T, int kLanes, int NV, int kEnd, bool kNt = false>
 __device__ __forceinline__ void load_row(const T *p, int cols, int lane, u32x4 (&raw)[NV]) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = (v * kLanes + lane) * kRowVec<T>;
-    raw[v] = row_load<T, kTail, kNt>(p + c, cols - c);
+    const int c = column<T, kLanes, kEnd>(cols, lane, v);
+    raw[v] = row_load<T, kEnd == kNarrow, kNt>(p + c, cols - c);
   }
 }
 
@@ -112,10 +133,10 @@ __device__ __forceinline__ void load_row(const T *p, int cols, int lane, u32x4 (
 // that the arithmetic behind it asks no questions.
 template <typename T>
 constexpr uint32_t kOnes = sizeof(T) == 4 ? 0x3f800000u : 0x3f803f80u;
-template <typename T, int kLanes, int NV, bool kTail, bool kNt = false>
+template <typename T, int kLanes, int NV, int kEnd, bool kNt = false>
 __device__ __forceinline__ void load_row_or(bool there, uint32_t bits, const T *p, int cols, int lane, u32x4 (&raw)[NV]) {
   if (there) {
-    load_row<T, kLanes, NV, kTail, kNt>(p, cols, lane, raw);
+    load_row<T, kLanes, NV, kEnd, kNt>(p, cols, lane, raw);
   } else {
 #pragma unroll
     for (int v = 0; v < NV; ++v) raw[v] = u32x4{bits, bits, bits, bits};
@@ -132,7 +153,7 @@ __device__ __forceinline__ void keep_packed(u32x4 (&raw)[NV]) {
 }
 
 // The row to `copies` members, `step` bytes apart.
-template <typename T, int kLanes, int NV, bool kTail>
+template <typename T, int kLanes, int NV, int kEnd>
 __device__ __forceinline__ void store_row(T *p, int64_t step, int copies, int cols, int lane,
                                           const float (&f)[NV][kRowVec<T>]) {
   u32x4 raw[NV];
@@ -141,8 +162,8 @@ __device__ __forceinline__ void store_row(T *p, int64_t step, int copies, int co
   for (int m = 0; m < copies; ++m) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * kLanes + lane) * kRowVec<T>;
-      row_store<T, kTail, true>(bytes_on(p, m * step) + c, cols - c, raw[v]);
+      const int c = column<T, kLanes, kEnd>(cols, lane, v);
+      row_store<T, kEnd == kNarrow, true>(bytes_on(p, m * step) + c, cols - c, raw[v]);
     }
   }
 }
@@ -150,7 +171,7 @@ __device__ __forceinline__ void store_row(T *p, int64_t step, int copies, int co
 template <int kLanes>
 constexpr int kWgLanes = kLanes < 256 ? 256 : kLanes;
 
-template <typename T, int kLanes, int NV, bool kTail, bool kNt>
+template <typename T, int kLanes, int NV, int kEnd, bool kNt>
 __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
   constexpr int V = kRowVec<T>;
   __shared__ float slots[2 * (kWgLanes<kLanes> / 64)];
@@ -164,22 +185,22 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
   const int64_t held = s.replicated ? row : row - owner * s.share;
 
   u32x4 x[NV], wpre[NV], wpost[NV], gate[NV];
-  load_row<T, kLanes, NV, kTail, kNt>(row_at<T>(p.residual, home, held, s.residual_ld, 0), s.cols, lane, x);
-  load_row_or<T, kLanes, NV, kTail>(p.pre_weight, 0u, row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, wpre);
-  load_row_or<T, kLanes, NV, kTail>(p.post_weight, 0u, row_at<T>(p.post_weight, home, 0, 0, 0), s.cols, lane, wpost);
-  load_row_or<T, kLanes, NV, kTail>(p.gate, kOnes<T>, row_at<T>(p.gate, home, row / s.rows_per_gate, s.cols, 0), s.cols,
+  load_row<T, kLanes, NV, kEnd, kNt>(row_at<T>(p.residual, home, held, s.residual_ld, 0), s.cols, lane, x);
+  load_row_or<T, kLanes, NV, kEnd>(p.pre_weight, 0u, row_at<T>(p.pre_weight, home, 0, 0, 0), s.cols, lane, wpre);
+  load_row_or<T, kLanes, NV, kEnd>(p.post_weight, 0u, row_at<T>(p.post_weight, home, 0, 0, 0), s.cols, lane, wpost);
+  load_row_or<T, kLanes, NV, kEnd>(p.gate, kOnes<T>, row_at<T>(p.gate, home, row / s.rows_per_gate, s.cols, 0), s.cols,
                                     lane, gate);
 
   float acc[NV][V];
-  fold_members<T, kLanes, NV, kTail, kNt>(s, s.members, p.source, row, s.partial_ld, lane, acc);
-  if (p.total) store_row<T, kLanes, NV, kTail>(row_at<T>(p.total, home, row - owner * s.share, s.cols, 0), 0, 1, s.cols, lane, acc);
+  fold_members<T, kLanes, NV, kEnd, kNt>(s, s.members, p.source, row, s.partial_ld, lane, acc);
+  if (p.total) store_row<T, kLanes, NV, kEnd>(row_at<T>(p.total, home, row - owner * s.share, s.cols, 0), 0, 1, s.cols, lane, acc);
 
   if (s.post) {
     float ss[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int e = 0; e < V; ++e) ss[0] = fmaf(acc[v][e], acc[v][e], ss[0]);
+      for (int e = 0; e < V; ++e) ss[0] = fmaf(acc[v][e], counted<T, kLanes, kEnd>(s.cols, lane, v, e, acc[v][e]), ss[0]);
     row_sums<kLanes>(ss, slots, turn);
     const float r = rsqrtf(fmaf(ss[0], s.inv_cols, s.eps));
 #pragma unroll
@@ -194,10 +215,12 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
     for (int e = 0; e < V; ++e) {
       const float z = acc[v][e] * row_get<T>(gate[v], e);
       acc[v][e] = fmaf(s.residual_scale, row_get<T>(x[v], e), s.block_scale * z);
-      ss[0] = fmaf(acc[v][e], acc[v][e], ss[0]);
+      ss[0] = fmaf(acc[v][e], counted<T, kLanes, kEnd>(s.cols, lane, v, e, acc[v][e]), ss[0]);
     }
-  store_row<T, kLanes, NV, kTail>(row_at<T>(p.residual_out, s.replicated ? 0 : home, held, s.residual_ld, 0), s.step,
-                                  s.replicated ? s.members : 1, s.cols, lane, acc);
+  // The row may be stored over what a shifted lane of another wave still loads.
+  if (kEnd == kShifted && kLanes > 64 && !s.post) __syncthreads();
+  store_row<T, kLanes, NV, kEnd>(row_at<T>(p.residual_out, s.replicated ? 0 : home, held, s.residual_ld, 0), s.step,
+                                 s.replicated ? s.members : 1, s.cols, lane, acc);
   if (!p.normed) return;
   row_sums<kLanes>(ss, slots, turn);
   const float r = rsqrtf(fmaf(ss[0], s.inv_cols, s.eps));
@@ -205,25 +228,16 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[v][e] *= r * (s.pre_offset + row_get<T>(wpre[v], e));
-  store_row<T, kLanes, NV, kTail>(row_at<T>(p.normed, 0, row, s.normed_ld, 0), s.step, s.members, s.cols, lane, acc);
+  store_row<T, kLanes, NV, kEnd>(row_at<T>(p.normed, 0, row, s.normed_ld, 0), s.step, s.members, s.cols, lane, acc);
 }
 
-// A lane's sums over the rows of its unit, as 32-bit floats to row `at` of an array.
-template <typename T, int kLanes, int NV>
-__device__ __forceinline__ void store_part(float *part, int64_t at, int ld, int cols, int lane, const float (&f)[NV][kRowVec<T>]) {
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int c = (v * kLanes + lane) * kRowVec<T>;
-#pragma unroll
-    for (int k = 0; k < kRowVec<T>; k += 4) {
-      // part_ld is a multiple of 4, so a group of four that begins inside the row stays inside it
-      if (c + k < cols)
-        *reinterpret_cast<float4 *>(part + at * ld + c + k) = float4{f[v][k], f[v][k + 1], f[v][k + 2], f[v][k + 3]};
-    }
-  }
+// Four floats of row `at` of an array of sums, from column c on if the row has it.  part_ld is a multiple
+// of 4, so that a narrow row's four stay inside the array.
+__device__ __forceinline__ void store_part(float *part, int64_t at, int ld, int cols, int c, float4 f) {
+  if (c < cols) row_store<float, false>(part + at * ld + c, 4, row_pack<float>({f.x, f.y, f.z, f.w}));
 }
 
-template <typename T, int kLanes, int NV, bool kTail, bool kNt>
+template <typename T, int kLanes, int NV, int kEnd, bool kNt>
 __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackward p) {
   constexpr int V = kRowVec<T>;
   __shared__ float slots[2 * 3 * (kWgLanes<kLanes> / 64)];
@@ -261,10 +275,10 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
   constexpr bool kTight = NV * V >= 16;
   u32x4 wpre[NV], wpost[NV], g[NV];
   auto load_pre = [&] {
-    load_row_or<T, kLanes, NV, kTail>(p.pre_weight, 0u, row_at<T>(p.pre_weight, 0, 0, 0, 0), s.cols, lane, wpre);
+    load_row_or<T, kLanes, NV, kEnd>(p.pre_weight, 0u, row_at<T>(p.pre_weight, 0, 0, 0, 0), s.cols, lane, wpre);
   };
   auto load_post = [&] {
-    load_row_or<T, kLanes, NV, kTail>(p.post_weight, 0u, row_at<T>(p.post_weight, 0, 0, 0, 0), s.cols, lane, wpost);
+    load_row_or<T, kLanes, NV, kEnd>(p.post_weight, 0u, row_at<T>(p.post_weight, 0, 0, 0, 0), s.cols, lane, wpost);
   };
   if constexpr (!kTight) {
     load_pre();
@@ -284,18 +298,18 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
     const int64_t held = s.replicated ? row : shared;
     const int gate_row = uniform(static_cast<int>(row) / s.rows_per_gate);
     u32x4 x[NV], tot[NV], din[NV];
-    load_row_or<T, kLanes, NV, kTail, kNt>(p.grad_normed, 0u, row_at<T>(p.residual_out, home, held, s.residual_ld, 0), s.cols,
+    load_row_or<T, kLanes, NV, kEnd, kNt>(p.grad_normed, 0u, row_at<T>(p.residual_out, home, held, s.residual_ld, 0), s.cols,
                                            lane, x);
-    load_row_or<T, kLanes, NV, kTail, kNt>(p.total, 0u, row_at<T>(p.total, home, shared, s.cols, 0), s.cols, lane, tot);
-    load_row_or<T, kLanes, NV, kTail, kNt>(p.grad_residual_out, 0u,
+    load_row_or<T, kLanes, NV, kEnd, kNt>(p.total, 0u, row_at<T>(p.total, home, shared, s.cols, 0), s.cols, lane, tot);
+    load_row_or<T, kLanes, NV, kEnd, kNt>(p.grad_residual_out, 0u,
                                            row_at<T>(p.grad_residual_out, home, held, s.residual_ld, 0), s.cols, lane, din);
     auto load_gate = [&] {
-      load_row_or<T, kLanes, NV, kTail>(p.gate, kOnes<T>, row_at<T>(p.gate, home, gate_row, s.cols, 0), s.cols, lane, g);
+      load_row_or<T, kLanes, NV, kEnd>(p.gate, kOnes<T>, row_at<T>(p.gate, home, gate_row, s.cols, 0), s.cols, lane, g);
     };
     if constexpr (!kTight) load_gate();
     float d[NV][V];
     if constexpr (kTight) load_pre();
-    fold_members<T, kLanes, NV, kTail, kNt, kTight ? 4 : kFoldDepth>(s, p.grad_normed ? s.members : 0, p.grad_normed, row,
+    fold_members<T, kLanes, NV, kEnd, kNt, kTight ? 4 : kFoldDepth>(s, p.grad_normed ? s.members : 0, p.grad_normed, row,
                                                                     s.normed_ld, lane, d);
     // sum x'^2, sum t x' and sum s^2 in one go: the second mean is r(x') times a plain sum
     float sums[3] = {0.f, 0.f, 0.f};
@@ -304,9 +318,10 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float xe = row_get<T>(x[v], e), se = row_get<T>(tot[v], e);
-        sums[0] = fmaf(xe, xe, sums[0]);
-        sums[1] = fmaf(d[v][e] * (s.pre_offset + row_get<T>(wpre[v], e)), xe, sums[1]);
-        sums[2] = fmaf(se, se, sums[2]);
+        const float xc = counted<T, kLanes, kEnd>(s.cols, lane, v, e, xe);
+        sums[0] = fmaf(xe, xc, sums[0]);
+        sums[1] = fmaf(d[v][e] * (s.pre_offset + row_get<T>(wpre[v], e)), xc, sums[1]);
+        sums[2] = fmaf(se, counted<T, kLanes, kEnd>(s.cols, lane, v, e, se), sums[2]);
       }
     row_sums<kLanes>(sums, slots, turn);
     keep_packed(x);
@@ -334,7 +349,7 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
       for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int e = 0; e < V; ++e) dx[v][e] = s.residual_scale * d[v][e];
-      store_row<T, kLanes, NV, kTail>(row_at<T>(p.grad_residual, s.replicated ? 0 : home, held, s.residual_ld, 0), s.step,
+      store_row<T, kLanes, NV, kEnd>(row_at<T>(p.grad_residual, s.replicated ? 0 : home, held, s.residual_ld, 0), s.step,
                                       s.replicated ? s.members : 1, s.cols, lane, dx);
     }
     // from here on d is f, and then q
@@ -354,7 +369,7 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
         f *= row_get<T>(g[v], e);
         to_post[e] = f * u;
         f *= w;
-        qs[0] = fmaf(f, u, qs[0]);
+        qs[0] = fmaf(counted<T, kLanes, kEnd>(s.cols, lane, v, e, f), u, qs[0]);
         d[v][e] = f;
       }
       if (p.part_post) add_to(sums_of[1], v, to_post);
@@ -368,16 +383,16 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
 #pragma unroll
         for (int e = 0; e < V; ++e) d[v][e] = r1 * fmaf(-mean_qu * r1, row_get<T>(tot[v], e), d[v][e]);
     }
-    store_row<T, kLanes, NV, kTail>(row_at<T>(p.grad_source, 0, row, s.partial_ld, 0), s.step, s.members, s.cols, lane, d);
+    store_row<T, kLanes, NV, kEnd>(row_at<T>(p.grad_source, 0, row, s.partial_ld, 0), s.step, s.members, s.cols, lane, d);
     if (p.direct && p.grad_gate && (row + 1 == last || (row + 1) % s.rows_per_gate == 0)) {
       for (int m = 0; m < s.members; ++m) {
         float *out = reinterpret_cast<float *>(p.grad_gate + m * s.step) + static_cast<int64_t>(gate_row) * s.cols;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const int c = (v * kLanes + lane) * V + e;
-            if (c < s.cols) out[c] = sum_gate[v][e];
+          for (int k = 0; k < V; k += 4) {
+            const int c = column<T, kLanes, kEnd>(s.cols, lane, v) + k;
+            row_store<float, kEnd == kNarrow, true>(out + c, s.cols - c, row_pack<float>({sum_gate[v][k], sum_gate[v][k + 1], sum_gate[v][k + 2], sum_gate[v][k + 3]}));
           }
       }
 #pragma unroll
@@ -386,18 +401,17 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
         for (int e = 0; e < V; ++e) sum_gate[v][e] = 0.f;
     }
   }
-  auto leave = [&](float *part, auto &of) {
+  auto leave = [&](float *part, auto of) {
+    if (!part) return;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int k = 0; k < V / 4; ++k) {
-        const int c = (v * kLanes + lane) * V + 4 * k;
-        if (c < s.cols) *reinterpret_cast<float4 *>(part + static_cast<int64_t>(unit) * p.part_ld + c) = of[v * (V / 4) + k][threadIdx.x];
-      }
+      for (int k = 0; k < V; k += 4)
+        store_part(part, unit, p.part_ld, s.cols, column<T, kLanes, kEnd>(s.cols, lane, v) + k, of(v, k));
   };
-  if (p.part_pre) leave(p.part_pre, sums_of[0]);
-  if (p.part_post) leave(p.part_post, sums_of[1]);
-  if (p.part_gate) store_part<T, kLanes, NV>(p.part_gate, unit, p.part_ld, s.cols, lane, sum_gate);
+  leave(p.part_pre, [&](int v, int k) { return sums_of[0][(v * V + k) / 4][threadIdx.x]; });
+  leave(p.part_post, [&](int v, int k) { return sums_of[1][(v * V + k) / 4][threadIdx.x]; });
+  leave(p.part_gate, [&](int v, int k) { return float4{sum_gate[v][k], sum_gate[v][k + 1], sum_gate[v][k + 2], sum_gate[v][k + 3]}; });
 }
 
 // The units' sums, added up in a fixed order: workgroup (x, y) makes columns 32 x .. 32 x + 31 of sum y
@@ -471,35 +485,38 @@ RowLanes lanes_for(int cols, int vec, bool backward) {
   return *c;
 }
 
-template <typename T, int kLanes, int NV, typename P, bool kTail, bool kNt>
+template <typename T, int kLanes, int NV, typename P, int kEnd, bool kNt>
 void launch_rows(const P &p, int units, hipStream_t stream) {
   const unsigned per_wg = kWgLanes<kLanes> / kLanes;
   const dim3 grid((static_cast<unsigned>(units) + per_wg - 1) / per_wg), block(kWgLanes<kLanes>);
   if constexpr (std::is_same<P, NormForward>::value)
-    hipLaunchKernelGGL((norm_kernel<T, kLanes, NV, kTail, kNt>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((norm_kernel<T, kLanes, NV, kEnd, kNt>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((norm_grad_kernel<T, kLanes, NV, kTail, kNt>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((norm_grad_kernel<T, kLanes, NV, kEnd, kNt>), grid, block, 0, stream, p);
 }
 
-// How a call goes: rows that end inside a vector, and operands that the Infinity Cache could not hold.
+// How a call goes: how its rows end, and whether the Infinity Cache could not hold its operands.
 struct Manner {
-  bool tail, once;
+  RowEnd end;
+  bool once;
 };
 
 template <typename T, int kLanes, int NV, typename P>
 void launch_lanes(const P &p, int units, Manner m, hipStream_t stream) {
-  if (m.tail) {
-    if (m.once) launch_rows<T, kLanes, NV, P, true, true>(p, units, stream);
-    else launch_rows<T, kLanes, NV, P, true, false>(p, units, stream);
-  } else {
-    if (m.once) launch_rows<T, kLanes, NV, P, false, true>(p, units, stream);
-    else launch_rows<T, kLanes, NV, P, false, false>(p, units, stream);
+  if (m.end == kWhole) {
+    if (m.once) launch_rows<T, kLanes, NV, P, kWhole, true>(p, units, stream);
+    else launch_rows<T, kLanes, NV, P, kWhole, false>(p, units, stream);
+  } else if (m.end == kShifted) {
+    if (m.once) launch_rows<T, kLanes, NV, P, kShifted, true>(p, units, stream);
+    else launch_rows<T, kLanes, NV, P, kShifted, false>(p, units, stream);
+  } else if constexpr (kLanes == 64 && NV == 1) {
+    launch_rows<T, kLanes, NV, P, kNarrow, false>(p, units, stream);
   }
 }
 
 template <typename T, typename P>
 void launch_for(const P &p, int units, RowLanes l, bool once, hipStream_t stream) {
-  const Manner m{p.s.cols % kRowVec<T> != 0, once};
+  const Manner m{p.s.cols < kRowVec<T> ? kNarrow : p.s.cols % kRowVec<T> ? kShifted : kWhole, once};
   constexpr bool kBackward = std::is_same<P, NormBackward>::value, kBf16 = sizeof(T) == 2;
   switch (l.lanes * 8 + l.vecs) {
     case 64 * 8 + 1: return launch_lanes<T, 64, 1>(p, units, m, stream);

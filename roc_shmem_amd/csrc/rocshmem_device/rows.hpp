@@ -74,23 +74,32 @@ __device__ __forceinline__ u32x4 row_pack(const float (&f)[kRowVec<T>]) {
   return v;
 }
 
+// The first `left` elements of a vector, fewer than all of them: in pieces of 8, 4 and 2 bytes.
+typedef uint32_t u32_a2 __attribute__((aligned(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+template <typename T>
+__device__ __forceinline__ void row_store_tail(T *p, int left, u32x4 v) {
+  const int bytes = left * static_cast<int>(sizeof(T));
+  char *q = reinterpret_cast<char *>(p);
+  if (bytes & 8) *reinterpret_cast<u32x2_a2 *>(q) = u32x2{v[0], v[1]};
+  if (bytes & 4) *reinterpret_cast<u32_a2 *>(q + (bytes & 8)) = bytes & 8 ? v[2] : v[0];
+  if (bytes & 2) {
+    uint32_t w = v[0];
+#pragma unroll
+    for (int k = 1; k < 4; ++k)
+      if ((bytes & 12) == 4 * k) w = v[k];
+    *reinterpret_cast<uint16_t *>(q + (bytes & 12)) = static_cast<uint16_t>(w);
+  }
+}
+
 template <typename T, bool kTail, bool kNt = false>
 __device__ __forceinline__ void row_store(T *p, int left, u32x4 v) {
   if (!kTail ? left > 0 : left >= kRowVec<T>) {
     if constexpr (kNt) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_a2 *>(p));
     else *reinterpret_cast<u32x4_a2 *>(p) = v;
   } else if (kTail && left > 0) {
-    if constexpr (sizeof(T) == 4) {
-      uint32_t *q = reinterpret_cast<uint32_t *>(p);
-#pragma unroll
-      for (int e = 0; e < 3; ++e)
-        if (e < left) q[e] = v[e];
-    } else {
-      uint16_t *q = reinterpret_cast<uint16_t *>(p);
-#pragma unroll
-      for (int e = 0; e < 7; ++e)
-        if (e < left) q[e] = static_cast<uint16_t>(e % 2 ? v[e / 2] >> 16 : v[e / 2]);
-    }
+    row_store_tail(p, left, v);
   }
 }
 
