@@ -604,8 +604,6 @@ __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(LogprobBackwar
     const int left = rest <= 0 ? 0 : rest < p.shard - at ? static_cast<int>(rest) : p.shard - at;
     const T *x = reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at;
     T *out = reinterpret_cast<T *>(p.grad_logits + member * p.step) + row * p.grad_ld + at;
-    // a wave whose vectors lie behind the line's end has nothing to do
-    const int wave0 = uniform(lane & ~63);
 #pragma unroll
     for (int k = 0; k < kGradDeep; ++k) {
       const int c = (k * kGradLanes + lane) * V;
@@ -616,7 +614,6 @@ __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(LogprobBackwar
 #pragma unroll
     for (int k = 0; k < kGradDeep; ++k) {
       const int c = (k * kGradLanes + lane) * V;
-      if ((k * kGradLanes + wave0) * V >= left) break;
       row_store<T, true, kNt>(out + c, left - c, grad_of<T>(p, r, raw[k], id + c));
     }
   }
@@ -872,7 +869,7 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   p.per_members = per(static_cast<unsigned>(p.members));
   // Short lines would leave a workgroup without enough to do for its start: 4096 x 1000 bf16 over 8 members
   // 173 us by lines and 16 numbered through.  Longer ones pay more for numbering (a row's numbers are
-  // read for every vector) than for waves that have nothing to do.
+  // read for every vector) than for lanes that have nothing to do.
   const bool packed = p.vecs < 512;
   const size_t lines = a.rows * p.members;
   const size_t wgs = packed ? (lines * p.vecs + most - 1) / most : lines * static_cast<size_t>(p.chunks);

@@ -416,8 +416,9 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
 
 // The units' sums, added up in a fixed order: workgroup (x, y) makes columns 32 x .. 32 x + 31 of sum y
 // (0: pre_weight, 1: post_weight, then the gate rows) and writes them to every member.  32 columns, so
-// that two sums of 4096 columns already make 256 workgroups, with 32 lanes to share a column's units.
-constexpr int kSumQuads = 8, kSumRanks = 256 / kSumQuads;
+// that two sums of 4096 columns already make 256 workgroups; 128 lanes share a column's units, which are
+// up to some thousand.
+constexpr int kSumQuads = 8, kSumRanks = 128, kSumFold = 16;
 struct PartSums {
   const float *part_pre, *part_post, *part_gate;
   char *grad_pre, *grad_post, *grad_gate;
@@ -425,7 +426,7 @@ struct PartSums {
   int64_t step;
 };
 
-__global__ void __launch_bounds__(256) part_sums_kernel(PartSums p) {
+__global__ void __launch_bounds__(kSumQuads * kSumRanks) part_sums_kernel(PartSums p) {
   __shared__ float4 sums[kSumRanks][kSumQuads];
   const int y = blockIdx.y;
   const float *part = y == 0 ? p.part_pre : y == 1 ? p.part_post : p.part_gate;
@@ -449,16 +450,24 @@ __global__ void __launch_bounds__(256) part_sums_kernel(PartSums p) {
       sum.w += a.w;
     }
   }
+  auto add_up = [&](int from, int to) {   // ranks from .. to - 1 onto rank `from`
+    for (int k = from + 1; k < to; ++k) {
+      const float4 a = sums[k][quad];
+      sum.x += a.x;
+      sum.y += a.y;
+      sum.z += a.z;
+      sum.w += a.w;
+    }
+  };
+  // by groups of kSumFold ranks first, then the groups
   sums[rank][quad] = sum;
   __syncthreads();
+  if (rank % kSumFold == 0) add_up(rank, rank + kSumFold);
+  __syncthreads();
+  if (rank % kSumFold == 0) sums[rank / kSumFold][quad] = sum;
+  __syncthreads();
   if (rank != 0 || c >= p.cols) return;
-  for (int k = 1; k < kSumRanks; ++k) {
-    const float4 a = sums[k][quad];
-    sum.x += a.x;
-    sum.y += a.y;
-    sum.z += a.z;
-    sum.w += a.w;
-  }
+  add_up(0, kSumRanks / kSumFold);
   const float each[4] = {sum.x, sum.y, sum.z, sum.w};
   for (int m = 0; m < p.members; ++m) {
     float *to = reinterpret_cast<float *>(out + m * p.step) + (y >= 2 ? static_cast<int64_t>(y - 2) * p.cols : 0);
@@ -607,8 +616,9 @@ struct GradPlan {
 GradPlan plan_of(const NormShape &s, int dtype, bool has_gate) {
   GradPlan g{};
   g.lanes = lanes_for(s.cols, dtype == RSM_BF16 ? 8 : 4, true);
-  // enough units to fill the chip's 256 compute units, no more: each leaves its sums behind
-  const int64_t target = g.lanes.lanes == 64 ? 4096 : 256 * (1024 / g.lanes.lanes);
+  // Enough units to fill the chip's 256 compute units, no more: each leaves its sums behind.  (Rows of a
+  // wave, 8192 x 64 bf16 over 8 members: 1024 units 26.6 us, 2048 21.2, 4096 21.8.)
+  const int64_t target = g.lanes.lanes == 64 ? 2048 : 256 * (1024 / g.lanes.lanes);
   const int64_t per_unit = (s.rows + target - 1) / target;
   const int64_t group = has_gate ? s.rows_per_gate : s.rows;
   g.part_ld = (s.cols + 3) & ~3;
@@ -772,7 +782,7 @@ int rsm_norm_to_all_grad(const rsm_norm_grad_args_t *args, void *stream) {
     r.members = s.members;
     r.step = s.step;
     const unsigned gates = p.part_gate ? static_cast<unsigned>(gate_rows(s)) : 0;
-    hipLaunchKernelGGL(part_sums_kernel, dim3((s.cols + 4 * kSumQuads - 1) / (4 * kSumQuads), 2 + gates), dim3(256), 0, st, r);
+    hipLaunchKernelGGL(part_sums_kernel, dim3((s.cols + 4 * kSumQuads - 1) / (4 * kSumQuads), 2 + gates), dim3(kSumQuads * kSumRanks), 0, st, r);
   }
   return rsm::after_launch(call);
 }
