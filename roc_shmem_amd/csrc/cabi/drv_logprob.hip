@@ -123,7 +123,9 @@ struct Batch {
       const int member = static_cast<int>(p.per_vecs ? __umulhi(j, p.per_vecs) : j);
       const int off = static_cast<int>(j - member * p.vecs) * kRowVec<T> + c % kRowVec<T>;
       const int rest = member < p.members ? elements_left(p, member, off) : 0;
-      return {reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + off, rest, member * p.shard + off};
+      // beyond the last member's part, where nothing is left, the id would not fit an int
+      const unsigned id = static_cast<unsigned>(member) * static_cast<unsigned>(p.shard) + static_cast<unsigned>(off);
+      return {reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + off, rest, static_cast<int>(id)};
     } else {
       return {part + c, left - c, id + c};
     }

@@ -257,6 +257,53 @@ def test_tokens_outside_the_vocabulary_raise_the_status_word():
             rs.roc_shmem_finalize()
 
 
+@pytest.mark.parametrize("vocab", [1000, 20000])     # lines of the gradient numbered through, and workgroups of their own
+def test_tokens_outside_the_vocabulary_have_no_gradient(vocab):
+    rs.roc_shmem_init(2, 64 << 20, 4, 1024)
+    try:
+        rows = 40
+        c = Case(rs.FLOAT, rows, vocab, 2, tokens=np.arange(rows))
+        lse = np.asarray(ref.logprob_forward(c.f64(), c.tokens, c.scale, 0)["lse"][0], dtype=np.float32)
+        lse, ones = c.numbers(lse, np.float32), c.numbers(np.ones(rows), np.float32)
+
+        def gradient(tokens):
+            g = Rows(rows, c.width, np.float32, c.ld)
+            args = rs.LogprobGradArgs(lse=lse, grad_logprob=ones, grad_logits=g, **{**c.fields, "tokens": c.numbers(tokens, np.int64)})
+            rs.roc_shmem_logprob_to_all_grad(args)
+            rs.synchronize()
+            return g.read(0), g.read(1)
+
+        whole = gradient(c.tokens)
+        assert rs.take_status() == 0
+        for row, token in ((0, vocab), (17, 1 << 40), (39, np.iinfo(np.int64).max), (5, -1), (6, np.iinfo(np.int64).min)):
+            tokens = c.tokens.copy()
+            tokens[row] = token
+            part = gradient(tokens)
+            assert rs.take_status() == (2 if token > 0 else 0)
+            for got, was in zip(part, whole):
+                assert not got[row].any()
+                assert np.array_equal(np.delete(got, row, 0), np.delete(was, row, 0))
+    finally:
+        rs.roc_shmem_finalize()
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_as_many_members_as_there_can_be(rows):
+    with runtime(128, heap_size=8 << 20):
+        for dtype in (rs.BF16, rs.FLOAT):
+            run_forward(Case(dtype, rows, 1000, 128, top_k=20))
+            run_backward(Case(dtype, rows, 1000, 128))
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_a_shard_longer_than_any_vocabulary(rows):
+    """The first member holds everything; the others' ids would lie past 2^31."""
+    with runtime(4):
+        for vocab in (5, 3000):
+            run_forward(Case(rs.BF16, rows, vocab, 4, shard=(1 << 30) - 1, top_k=5))
+            run_backward(Case(rs.BF16, rows, vocab, 4, shard=(1 << 30) - 1))
+
+
 def test_each_result_alone():
     with runtime(4):
         for rows in (2, 260):

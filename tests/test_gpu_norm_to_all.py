@@ -240,6 +240,24 @@ def test_results_in_place_of_operands(dtype, replicated):
         run_backward(Case(dtype, 21, 1500, 4, replicated=replicated, gate=5), in_place=True)
 
 
+@pytest.mark.parametrize("cols", [5, 100, 1500, 2051, 8190])
+@pytest.mark.parametrize("dtype", [rs.BF16, rs.FLOAT])
+def test_rows_that_end_inside_a_vector_in_place(dtype, cols):
+    """Without a norm of the sum a row's new residual stream is stored soonest after its loads."""
+    with runtime(3):
+        for gate in (0, 4):
+            for replicated in (False, True):
+                run_forward(Case(dtype, 13, cols, 3, gate=gate, post=False, replicated=replicated), in_place=True)
+                run_backward(Case(dtype, 13, cols, 3, gate=gate, post=False, replicated=replicated), in_place=True)
+
+
+def test_as_many_members_as_there_can_be():
+    with runtime(128, heap_size=8 << 20):
+        for rows in (1, 130, 300):      # most members own nothing, one row, three
+            run_forward(Case(rs.BF16, rows, 72, 128, gate=0))
+            run_backward(Case(rs.FLOAT, rows, 72, 128, gate=0))
+
+
 def test_optional_operands():
     with runtime(4):
         run_forward(Case(rs.BF16, 12, 520, 4), keep=False)
