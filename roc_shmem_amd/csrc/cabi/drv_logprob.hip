@@ -132,17 +132,19 @@ struct Batch {
   }
 };
 
-// One batch of a wave.  Returns the largest of this lane's elements.
 template <typename T, bool kNt, bool kPacked>
-__device__ __forceinline__ float take_batch(const Batch<T, kPacked> &batch, float c2, Softmax &a) {
-  constexpr int V = kRowVec<T>;
-  const int lane = lane_id();
-  u32x4 raw[kDeep];
+__device__ __forceinline__ void load_batch(const Batch<T, kPacked> &batch, u32x4 (&raw)[kDeep]) {
 #pragma unroll
   for (int k = 0; k < kDeep; ++k) {
-    const Place<T> v = batch.at((k * 64 + lane) * V);
+    const Place<T> v = batch.at((k * 64 + lane_id()) * kRowVec<T>);
     raw[k] = row_load<T, true, kNt>(v.p, v.left, kMinusInf<T>);
   }
+}
+
+// One batch of a wave.  Returns the largest of this lane's elements.
+template <typename T>
+__device__ __forceinline__ float take_batch(const u32x4 (&raw)[kDeep], float c2, Softmax &a) {
+  constexpr int V = kRowVec<T>;
   float best = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kDeep; ++k)
@@ -342,8 +344,10 @@ __device__ __forceinline__ float element_at(const Place<T> &v) {
 }
 
 // 64 vector registers at most, so that a compute unit holds four workgroups: while some rank their
-// row's alternatives the others stream.
-template <typename T, bool kTop, bool kNt, bool kPacked>
+// row's alternatives the others stream.  kSingle: no wave has more than one batch of alternatives to look
+// at, which then stays in its registers (4096 x 16000 bf16, 8 alternatives: 42 us against 47; one row of 128000
+// over 8 members, 20 of them: 10.6 against 11.2).
+template <typename T, bool kTop, bool kNt, bool kPacked, bool kSingle>
 __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForward p) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = lane_id(), wave = uniform(static_cast<int>(threadIdx.x / 64)), waves = blockDim.x / 64;
@@ -358,8 +362,17 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
   const int per_note = ((end - first + waves - 1) / waves + kNotes - 1) / kNotes;
   float best = -INFINITY, note = -INFINITY;
   int turn = 0, at_note = 0;
-  for (int b = first + wave; b < end; b += waves) {
-    const float here = take_batch<T, kNt>(Batch<T, kPacked>(p, row, b), c2, a);
+  u32x4 kept[kDeep];   // kSingle: the wave's only batch
+  if constexpr (kSingle) {
+    if (first + wave < end) {
+      load_batch<T, kNt>(Batch<T, kPacked>(p, row, first + wave), kept);
+      best = take_batch<T>(kept, c2, a);
+    }
+  }
+  for (int b = first + wave; !kSingle && b < end; b += waves) {
+    u32x4 raw[kDeep];
+    load_batch<T, kNt>(Batch<T, kPacked>(p, row, b), raw);
+    const float here = take_batch<T>(raw, c2, a);
     if constexpr (kTop) {
       best = fmaxf(best, here);
       note = fmaxf(note, here);
@@ -381,13 +394,28 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
     if constexpr (kTop) sh.best[wave][lane] = best;
     __syncthreads();
     if constexpr (kTop) {
+      const float here = best;
       for (int w = 0; w < waves; ++w) best = fmaxf(best, sh.best[w][lane]);
       const uint32_t order = bound_of_lanes(order_of(best), p.top_k);
       const bool bounded = order > kOrderOfMinusInf;
       const float bound = bounded ? value_of_order(order) : kLowest;
       int n = 0;
+      auto gather = [&](const Batch<T, kPacked> &batch, const u32x4 (&raw)[kDeep]) {
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k) {
+          const int id = batch.at((k * 64 + lane) * kRowVec<T>).id;
+#pragma unroll
+          for (int e = 0; e < kRowVec<T>; ++e) {
+            const float x = row_get<T>(raw[k], e);
+            found_add(sh.found[wave], n, x >= bound, key_of(x, id + e));
+          }
+        }
+      };
+      if constexpr (kSingle) {
+        if (__ballot(here >= bound)) gather(Batch<T, kPacked>(p, row, first + wave), kept);
+      }
       turn = at_note = 0;
-      for (int b = first + wave; b < end && n <= kRoom; b += waves) {
+      for (int b = first + wave; !kSingle && b < end && n <= kRoom; b += waves) {
         const bool near = sh.notes[wave][at_note][lane] >= bound;
         if (++turn == per_note) {
           turn = 0;
@@ -396,20 +424,12 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
         if (!__ballot(near)) continue;
         const Batch<T, kPacked> batch(p, row, b);
         u32x4 raw[kDeep];
-        int id[kDeep];
 #pragma unroll
         for (int k = 0; k < kDeep; ++k) {
           const Place<T> v = batch.at((k * 64 + lane) * kRowVec<T>);
-          id[k] = v.id;
           raw[k] = row_load<T, true>(v.p, near ? v.left : 0, kMinusInf<T>);
         }
-#pragma unroll
-        for (int k = 0; k < kDeep; ++k)
-#pragma unroll
-          for (int e = 0; e < kRowVec<T>; ++e) {
-            const float x = row_get<T>(raw[k], e);
-            found_add(sh.found[wave], n, x >= bound, key_of(x, id[k] + e));
-          }
+        gather(batch, raw);
       }
       if (lane == 0) sh.count[wave] = n;
       __syncthreads();
@@ -421,7 +441,7 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
         // above minus infinity (room) only elements at minus infinity are missing.
         for (int b = first; b < end && !(room && t.last != 0); ++b) {
           const int w = (b - first) % waves, i = (b - first) / waves;
-          const uint32_t noted = order_of(sh.notes[w][i / per_note][lane] + 0.f);
+          const uint32_t noted = order_of((kSingle ? sh.best[w][lane] : sh.notes[w][i / per_note][lane]) + 0.f);
           if (!__ballot(noted > static_cast<uint32_t>(t.last >> 32))) continue;
           const Batch<T, kPacked> batch(p, row, b);
           for (int e = 0; e < kBatch<T> / 64; ++e) {
@@ -676,13 +696,14 @@ LogprobPlan plan_of(const LogprobShape &s, int dtype, size_t rows, size_t vocab,
                                : static_cast<int64_t>(members) * g.batches_per_member;
   g.batches = static_cast<int>(all);
   g.parts = 1;
-  // Few rows: several workgroups to a row, so that the chip has some 512 to run, each with four batches
-  // at least, one for each of its waves: then a SIMD has one wave to run.  More and smaller ones lose more
-  // in the joining than they win (one row of 128000 bf16 with 20 alternatives: 8 workgroups of 8 waves
-  // 11.3 us, 16 of 4 10.9, 32 of 2 11.3; 64 x 50257 float with 5: 512 workgroups 11.6, 1024 12.2).
+  // Few rows: several workgroups to a row, so that the chip has some 1024 to run, four to a compute unit, but
+  // each with eight batches, one for each of its waves, which then ranks them without reading them again.
+  // Smaller shares lose more in the joining than they win, larger ones leave memory idle (512 workgroups of
+  // four batches and more against 1024 of eight, 4 alternatives: 1 x 128000 bf16 over 8 members 10.7 and 10.3
+  // us, 64 x 152000 15.4 and 13.7, 200 x 152000 25.2 and 23.1; 1 x 32000 9.3 and 9.7, 128 x 152000 18.8 and 19.6).
   if (rows && rows < 256) {
-    int64_t parts = 512 / static_cast<int64_t>(rows);
-    const int64_t most = (all + 3) / 4;
+    int64_t parts = 1024 / static_cast<int64_t>(rows);
+    const int64_t most = (all + kMaxWaves - 1) / kMaxWaves;
     if (parts > most) parts = most;
     if (parts > kMaxParts) parts = kMaxParts;
     g.parts = parts < 1 ? 1 : static_cast<int>(parts);
@@ -704,8 +725,11 @@ template <typename T, bool kTop, bool kNt>
 void launch_forward(const LogprobForward &p, bool packed, dim3 grid, int waves, hipStream_t st) {
   const dim3 block(static_cast<unsigned>(waves * 64));
   const size_t lds = shared_bytes(waves, kTop);
-  if (packed) hipLaunchKernelGGL((logprob_kernel<T, kTop, kNt, true>), grid, block, lds, st, p);
-  else hipLaunchKernelGGL((logprob_kernel<T, kTop, kNt, false>), grid, block, lds, st, p);
+  const bool single = kTop && (p.batches + p.parts - 1) / p.parts <= waves;
+  if (single && packed) hipLaunchKernelGGL((logprob_kernel<T, kTop, kNt, true, kTop>), grid, block, lds, st, p);
+  else if (single) hipLaunchKernelGGL((logprob_kernel<T, kTop, kNt, false, kTop>), grid, block, lds, st, p);
+  else if (packed) hipLaunchKernelGGL((logprob_kernel<T, kTop, kNt, true, false>), grid, block, lds, st, p);
+  else hipLaunchKernelGGL((logprob_kernel<T, kTop, kNt, false, false>), grid, block, lds, st, p);
 }
 
 template <typename T>

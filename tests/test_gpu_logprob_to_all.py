@@ -185,6 +185,21 @@ def test_masks(dtype, rows, vocab):
             run_backward(c)
 
 
+@pytest.mark.parametrize("dtype", [rs.BF16, rs.FLOAT])
+def test_several_workgroups_to_a_row_of_several_batches_each(dtype):
+    rows, vocab = 255, 80001
+    rng = np.random.default_rng(4)
+    base = rng.standard_normal((rows, vocab)) * 2
+    base[40:80] = np.where(rng.random((40, vocab)) < 0.5, -np.inf, base[40:80])
+    base[80:100] = np.round(base[80:100])
+    base[100:105] = 1.5
+    base[105:110] = np.where(np.arange(vocab) % 5000 == 17, base[105:110], -np.inf)
+    base[110] = -np.inf
+    base[111] = np.where(np.arange(vocab) == vocab - 1, 0.5, -np.inf)
+    with runtime(3, heap_size=128 << 20):
+        run_forward(Case(dtype, rows, vocab, 3, logits=base, top_k=20, tokens=rng.integers(0, vocab, rows)), times=2)
+
+
 def test_rows_at_the_lowest_value_are_uniform():
     """Logits that are all the type's lowest value are equal like any others; the normaliser itself,
     lowest + ln V, is the lowest value as a float."""
