@@ -132,6 +132,19 @@ struct Batch {
   }
 };
 
+// The same for a batch of each lane's own.
+template <typename T, bool kPacked>
+__device__ __forceinline__ Place<T> place_in(const LogprobForward &p, int row, int b, int c) {
+  if constexpr (kPacked) {
+    return Batch<T, true>(p, row, b).at(c);
+  } else {
+    const int member = static_cast<int>(static_cast<unsigned>(b) / static_cast<unsigned>(p.batches_per_member));
+    const int at = (b - member * p.batches_per_member) * kBatch<T> + c;
+    return {reinterpret_cast<const T *>(p.logits + member * p.step) + row * p.ld + at, elements_left(p, member, at),
+            static_cast<int>(static_cast<int64_t>(member) * p.shard + at)};
+  }
+}
+
 template <typename T, bool kNt, bool kPacked>
 __device__ __forceinline__ void load_batch(const Batch<T, kPacked> &batch, u32x4 (&raw)[kDeep]) {
 #pragma unroll
@@ -400,36 +413,56 @@ __global__ void __launch_bounds__(kMaxWaves * 64, 8) logprob_kernel(LogprobForwa
       const bool bounded = order > kOrderOfMinusInf;
       const float bound = bounded ? value_of_order(order) : kLowest;
       int n = 0;
-      auto gather = [&](const Batch<T, kPacked> &batch, const u32x4 (&raw)[kDeep]) {
+      auto gather = [&](const u32x4 (&raw)[kDeep], const int (&id)[kDeep]) {
 #pragma unroll
-        for (int k = 0; k < kDeep; ++k) {
-          const int id = batch.at((k * 64 + lane) * kRowVec<T>).id;
+        for (int k = 0; k < kDeep; ++k)
 #pragma unroll
           for (int e = 0; e < kRowVec<T>; ++e) {
             const float x = row_get<T>(raw[k], e);
-            found_add(sh.found[wave], n, x >= bound, key_of(x, id + e));
+            found_add(sh.found[wave], n, x >= bound, key_of(x, id[k] + e));
           }
-        }
       };
       if constexpr (kSingle) {
-        if (__ballot(here >= bound)) gather(Batch<T, kPacked>(p, row, first + wave), kept);
-      }
-      turn = at_note = 0;
-      for (int b = first + wave; !kSingle && b < end && n <= kRoom; b += waves) {
-        const bool near = sh.notes[wave][at_note][lane] >= bound;
-        if (++turn == per_note) {
-          turn = 0;
-          ++at_note;
-        }
-        if (!__ballot(near)) continue;
-        const Batch<T, kPacked> batch(p, row, b);
-        u32x4 raw[kDeep];
+        if (__ballot(here >= bound)) {
+          const Batch<T, kPacked> batch(p, row, first + wave);
+          int id[kDeep];
 #pragma unroll
-        for (int k = 0; k < kDeep; ++k) {
-          const Place<T> v = batch.at((k * 64 + lane) * kRowVec<T>);
-          raw[k] = row_load<T, true>(v.p, near ? v.left : 0, kMinusInf<T>);
+          for (int k = 0; k < kDeep; ++k) id[k] = batch.at((k * 64 + lane) * kRowVec<T>).id;
+          gather(kept, id);
         }
-        gather(batch, raw);
+      } else {
+        // What is near the bound, a lane's vectors of a batch each, is read by 64 lanes at a time, so that
+        // the wave waits for memory once and not for every batch: lane r holds the r-th of them.
+        int near_ones = 0, one = 0;
+        auto look = [&] {
+          u32x4 raw[kDeep];
+          int id[kDeep];
+#pragma unroll
+          for (int k = 0; k < kDeep; ++k) {
+            const Place<T> v = place_in<T, kPacked>(p, row, one >> 6, (k * 64 + (one & 63)) * kRowVec<T>);
+            id[k] = v.id;
+            raw[k] = row_load<T, true>(v.p, lane < near_ones ? v.left : 0, kMinusInf<T>);
+          }
+          gather(raw, id);
+          near_ones = 0;
+        };
+        turn = at_note = 0;
+        for (int b = first + wave; b < end && n <= kRoom; b += waves) {
+          const uint64_t near = __ballot(sh.notes[wave][at_note][lane] >= bound);
+          if (++turn == per_note) {
+            turn = 0;
+            ++at_note;
+          }
+          if (near == 0) continue;
+          const int more = __popcll(near), below = rank_in_mask(near);
+          if (near_ones + more > 64) look();
+          // to the free lanes in order, the others' behind them
+          const int to = near_ones + (near >> lane & 1 ? below : more + lane - below);
+          const int sent = __builtin_amdgcn_ds_permute((to & 63) * 4, b << 6 | lane);
+          if (lane >= near_ones && lane < near_ones + more) one = sent;
+          near_ones += more;
+        }
+        if (near_ones > 0 && n <= kRoom) look();
       }
       if (lane == 0) sh.count[wave] = n;
       __syncthreads();
