@@ -200,6 +200,19 @@ def test_several_workgroups_to_a_row_of_several_batches_each(dtype):
         run_forward(Case(dtype, rows, vocab, 3, logits=base, top_k=20, tokens=rng.integers(0, vocab, rows)), times=2)
 
 
+@pytest.mark.parametrize("vocab", [9000, 20000])
+def test_many_rows_that_are_not_long(vocab):
+    """Workgroups of half as many waves, with one batch each or several."""
+    rows = 2050
+    rng = np.random.default_rng(6)
+    base = rng.standard_normal((rows, vocab)) * 2
+    base[::7] = np.round(base[::7])
+    base[::50] = -1.5
+    base[1::50, 30:] = -np.inf
+    with runtime(2, heap_size=128 << 20):
+        run_forward(Case(rs.BF16, rows, vocab, 2, logits=base, top_k=9, tokens=rng.integers(0, vocab, rows)))
+
+
 def test_rows_at_the_lowest_value_are_uniform():
     """Logits that are all the type's lowest value are equal like any others; the normaliser itself,
     lowest + ln V, is the lowest value as a float."""
