@@ -325,7 +325,8 @@ enum rsm_norm_flags {
  * member's is written.  `total` (may be NULL) keeps s for the backward pass: share rows, packed, on the
  * owners.  The weights (cols elements) and `gate` (one packed row for every rows_per_gate rows of the
  * batch; 0 = one row for all) hold the same values on every member.  `normed` may be NULL, may be
- * `source` (equal strides), and residual_out may be `residual`.  cols <= 16384, rows < 2^22, eps > 0. */
+ * `source` (equal strides), and residual_out may be `residual`.  cols <= 16384, rows < 2^22, eps a positive
+ * normal float.  Means of squares are 32-bit floats: a row whose mean square overflows comes out as zeros. */
 typedef struct rsm_norm_args {
   int dtype;
   int flags;                 /* rsm_norm_flags */
@@ -344,10 +345,10 @@ int rsm_norm_to_all(const rsm_norm_args_t *args, void *stream);
  * left (total: needed with RSM_NORM_POST and for grad_gate).  Results: grad_source, the gradient of every
  * member's part, the same on all of them; grad_residual (may be NULL), held as the stream is; and,
  * where they are not NULL, 32-bit sums over the rows on every member: grad_pre_weight and
- * grad_post_weight (cols floats), grad_gate (gate's shape).  grad_source may be grad_normed (equal
+ * grad_post_weight (cols floats), grad_gate (gate's shape, packed floats).  grad_source may be grad_normed (equal
  * strides) and grad_residual may be grad_residual_out.  `work`: rsm_norm_grad_work_bytes() bytes of a
- * symmetric array that no other call in flight uses (the first member's copy is written); not needed
- * when none of the sums is asked for.  normed_ld: grad_normed's, source_ld: grad_source's,
+ * symmetric array, aligned to 16 bytes, that no other call in flight uses (the first member's copy is
+ * written); not needed when none of the sums is asked for.  normed_ld: grad_normed's, source_ld: grad_source's,
  * residual_ld: the stream's arrays'. */
 typedef struct rsm_norm_grad_args {
   int dtype;
@@ -376,10 +377,10 @@ int rsm_norm_grad_work_bytes(const rsm_norm_grad_args_t *args, size_t *bytes);
  * outside the vocabulary; a row of nothing else has lse and log probabilities of minus infinity and
  * entropy 0.  A row with a NaN or plus infinity has NaN results; NaN logits are never alternatives, and
  * where fewer than top_k others are there the rest of the row is id -1 with NaN.
- * `work` (rsm_logprob_work_bytes() bytes) and pSync (ROC_SHMEM_REDUCE_SYNC_SIZE longs, all
+ * `work` (rsm_logprob_work_bytes() bytes, aligned to 16) and pSync (ROC_SHMEM_REDUCE_SYNC_SIZE longs, all
  * ROC_SHMEM_SYNC_VALUE on entry and on return) are symmetric arrays that no other call in flight uses;
  * the first member's copies serve batches of fewer than 256 rows, and larger ones need neither (0
- * bytes).  rows < 2^22, vocab < 2^30, scale > 0. */
+ * bytes).  rows < 2^22, vocab < 2^30, scale a positive normal float below 2^127. */
 typedef struct rsm_logprob_args {
   int dtype;
   int top_k;

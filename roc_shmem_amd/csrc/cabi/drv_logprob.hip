@@ -356,6 +356,10 @@ __device__ __forceinline__ float element_at(const Place<T> &v) {
   else return bf16_bits_to_float(*reinterpret_cast<const uint16_t *>(v.p));
 }
 
+// Without alternatives the stream of logits bounds it: 4096 x 131072 bf16 over 8 members 164 us, 6.5 TB/s, as
+// for half as many float ones; with 8 of them 185.  One row of 128000 over 8 members with 20 takes 10 us, a chain
+// of phases: 2 to stream, 3 to bound and rank, 3 to join the workgroups, 1 to write.
+//
 // 64 vector registers at most, so that a compute unit holds four workgroups: while some rank their
 // row's alternatives the others stream.  kSingle: no wave has more than one batch of alternatives to look
 // at, which then stays in its registers (4096 x 16000 bf16, 8 alternatives: 42 us against 47; one row of 128000
