@@ -323,6 +323,13 @@ def test_as_many_members_as_there_can_be(rows):
             run_backward(Case(dtype, rows, 1000, 128))
 
 
+def test_as_many_rows_as_there_can_be():
+    with runtime(1, heap_size=1 << 30):
+        c = Case(rs.BF16, (1 << 22) - 1, 6, 1)
+        run_forward(c)
+        run_backward(c)
+
+
 @pytest.mark.parametrize("rows", [3, 300])
 def test_a_shard_longer_than_any_vocabulary(rows):
     """The first member holds everything; the others' ids would lie past 2^31."""

@@ -258,6 +258,12 @@ def test_as_many_members_as_there_can_be():
             run_backward(Case(rs.FLOAT, rows, 72, 128, gate=0))
 
 
+def test_as_many_rows_as_there_can_be():
+    with runtime(1, heap_size=1 << 30):
+        run_forward(Case(rs.BF16, (1 << 22) - 1, 8, 1, gate=0))
+        run_backward(Case(rs.BF16, (1 << 22) - 1, 8, 1, gate=0, post=False), sums=False)
+
+
 def test_optional_operands():
     with runtime(4):
         run_forward(Case(rs.BF16, 12, 520, 4), keep=False)
