@@ -327,6 +327,12 @@ def test_gate_gradients_where_units_hold_many_rows(rows_per_gate):
         run_backward(Case(rs.BF16, 2100, 1100, 2, gate=rows_per_gate, seed=rows_per_gate))
 
 
+@pytest.mark.parametrize("gate", [0, 1, 3, 700])
+def test_many_rows_of_many_members(gate):
+    with runtime(5, heap_size=128 << 20):
+        run_backward(Case(rs.BF16, 1501, 1100, 5, gate=gate, seed=gate))
+
+
 def test_no_rows():
     with runtime(4):
         run_forward(Case(rs.BF16, 0, 100, 4, gate=0))
