@@ -324,9 +324,9 @@ enum rsm_norm_flags {
  * RSM_NORM_REPLICATED the arrays have all rows on every member, the owner's copy is read and every
  * member's is written.  `total` (may be NULL) keeps s for the backward pass: share rows, packed, on the
  * owners.  The weights (cols elements) and `gate` (one packed row for every rows_per_gate rows of the
- * batch; 0 = one row for all) hold the same values on every member.  `normed` may be NULL, may be
- * `source` (equal strides), and residual_out may be `residual`.  cols <= 16384, rows < 2^22, eps a positive
- * normal float.  Means of squares are 32-bit floats: a row whose mean square overflows comes out as zeros. */
+ * batch; 0 = one row for all; without a gate the field is not looked at) hold the same values on every
+ * member.  `normed` may be NULL, may be `source` (equal strides), and residual_out may be `residual`.
+ * cols <= 16384, rows < 2^22, eps a positive normal float.  Means of squares are 32-bit floats: a row whose mean square overflows comes out as zeros. */
 typedef struct rsm_norm_args {
   int dtype;
   int flags;                 /* rsm_norm_flags */

@@ -593,7 +593,9 @@ bool shape_of(const A &a, const char *call, size_t partial_ld, size_t normed_ld,
   s.members = team.size;
   s.share = static_cast<int>((a.rows + team.size - 1) / team.size);
   if (s.share < 1) s.share = 1;
-  s.rows_per_gate = a.rows_per_gate == 0 || a.rows_per_gate > a.rows ? (s.rows ? s.rows : 1) : static_cast<int>(a.rows_per_gate);
+  // without a gate all rows are one group, whatever the field says
+  const bool one_group = !a.gate || a.rows_per_gate == 0 || a.rows_per_gate > a.rows;
+  s.rows_per_gate = one_group ? (s.rows ? s.rows : 1) : static_cast<int>(a.rows_per_gate);
   s.step = team.step;
   s.partial_ld = static_cast<int64_t>(partial_ld);
   s.normed_ld = static_cast<int64_t>(normed_ld);
@@ -631,7 +633,7 @@ GradPlan plan_of(const NormShape &s, int dtype, bool has_gate) {
   // members 162 and 167, over 1 98 and 109.)
   const int64_t target = g.lanes.lanes == 64 ? 2048 : g.lanes.lanes == 256 && s.members < 4 ? 1024 : g.lanes.lanes == 1024 ? 256 : 512;
   const int64_t per_unit = (s.rows + target - 1) / target;
-  const int64_t group = has_gate ? s.rows_per_gate : s.rows;
+  const int64_t group = s.rows_per_gate;
   g.part_ld = (s.cols + 3) & ~3;
   if (group <= per_unit && has_gate && gate_rows(s) > 1) {
     g.direct = true;
@@ -642,8 +644,7 @@ GradPlan plan_of(const NormShape &s, int dtype, bool has_gate) {
     g.direct = false;
     g.units_per_gate = static_cast<int>((group + per_unit - 1) / (per_unit ? per_unit : 1));
     if (g.units_per_gate < 1) g.units_per_gate = 1;
-    g.rows_per_unit = static_cast<int>((group + g.units_per_gate - 1) / g.units_per_gate);
-    g.units = g.units_per_gate * static_cast<int>(has_gate ? gate_rows(s) : s.rows ? 1 : 0);
+    g.units = g.units_per_gate * static_cast<int>(gate_rows(s));
   }
   g.parts = 1 + (s.post ? 1 : 0) + (has_gate && !g.direct ? 1 : 0);
   g.part_bytes = static_cast<size_t>(g.units) * g.part_ld * sizeof(float);

@@ -1,0 +1,24 @@
+"""Row collectives at the edges of their contract."""
+import pytest
+
+import roc_shmem_amd as rs
+from helpers import runtime
+from test_gpu_norm_to_all import Case as NormCase
+from test_gpu_norm_to_all import run_backward, run_forward
+
+pytestmark = pytest.mark.gpu
+
+BOTH = pytest.mark.parametrize("dtype", [rs.BF16, rs.FLOAT])
+
+
+@BOTH
+@pytest.mark.parametrize("rows,cols,rows_per_gate", [(100, 72, 1), (100, 72, 10), (100, 72, 99), (100, 72, 100), (100, 72, 1000),
+                                                     (37, 1031, 5), (2100, 1100, 1), (2100, 1100, 700), (2100, 1100, 2101)])
+def test_rows_per_gate_means_nothing_without_a_gate(dtype, rows, cols, rows_per_gate):
+    """Every row has its gradient and counts in the weights' sums, whether a unit walks one row or several."""
+    for replicated in (False, True):
+        with runtime(2, heap_size=256 << 20):
+            c = NormCase(dtype, rows, cols, 2, gate=0, replicated=replicated, seed=rows_per_gate)
+            c.fields["rows_per_gate"] = rows_per_gate
+            run_forward(c)
+            run_backward(c)
