@@ -910,8 +910,7 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   o.add(a.grad_logprob, "grad_logprob", a.rows * 4, 4, false);
   o.add(a.grad_entropy, "grad_entropy", a.rows * 4, 4, false);
   o.add(a.grad_lse, "grad_lse", a.rows * 4, 4, false);
-  o.matrix(a.grad_logits, "grad_logits", a.rows, width, grad_ld, size, true);
-  if (grad_ld == s.ld) o.or_same_as(a.logits);
+  o.matrix(a.grad_logits, "grad_logits", a.rows, width, grad_ld, size, true, grad_ld == s.ld ? a.logits : nullptr);
   if (!o.ok()) return -1;
   LogprobBackward p{};
   p.rows = static_cast<int>(a.rows);

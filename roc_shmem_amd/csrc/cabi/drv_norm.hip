@@ -682,10 +682,8 @@ int rsm_norm_to_all(const rsm_norm_args_t *args, void *stream) {
   o.add(a.pre_weight, "pre_weight", a.cols * size, size, false);
   o.add(a.post_weight, "post_weight", a.cols * size, size, false);
   o.add(a.gate, "gate", gate_rows(s) * a.cols * size, size, false);
-  o.matrix(a.residual_out, "residual_out", held, a.cols, ld, size, true);
-  o.or_same_as(a.residual);
-  o.matrix(a.normed, "normed", a.rows, a.cols, normed_ld, size, true);
-  if (normed_ld == source_ld) o.or_same_as(a.source);
+  o.matrix(a.residual_out, "residual_out", held, a.cols, ld, size, true, a.residual);
+  o.matrix(a.normed, "normed", a.rows, a.cols, normed_ld, size, true, normed_ld == source_ld ? a.source : nullptr);
   o.matrix(a.total, "total", s.share, a.cols, a.cols, size, true);
   if (!o.ok()) return -1;
   NormForward p{};
@@ -744,10 +742,8 @@ int rsm_norm_to_all_grad(const rsm_norm_grad_args_t *args, void *stream) {
   o.add(a.pre_weight, "pre_weight", a.cols * size, size, false);
   o.add(a.post_weight, "post_weight", a.cols * size, size, false);
   o.add(a.gate, "gate", gate_rows(s) * a.cols * size, size, false);
-  o.matrix(a.grad_source, "grad_source", a.rows, a.cols, source_ld, size, true);
-  if (source_ld == normed_ld) o.or_same_as(a.grad_normed);
-  o.matrix(a.grad_residual, "grad_residual", mine, a.cols, ld, size, true);
-  o.or_same_as(a.grad_residual_out);
+  o.matrix(a.grad_source, "grad_source", a.rows, a.cols, source_ld, size, true, source_ld == normed_ld ? a.grad_normed : nullptr);
+  o.matrix(a.grad_residual, "grad_residual", mine, a.cols, ld, size, true, a.grad_residual_out);
   o.add(a.grad_pre_weight, "grad_pre_weight", a.cols * 4, 4, true);
   o.add(a.grad_post_weight, "grad_post_weight", a.cols * 4, 4, true);
   o.add(a.grad_gate, "grad_gate", gate_rows(s) * a.cols * 4, 4, true);

@@ -25,17 +25,15 @@ class Operands {
  public:
   explicit Operands(const char *call) : call_(call) {}
 
-  // rows x cols elements of `size` bytes, `ld` elements from row to row.
-  void matrix(const void *p, const char *name, size_t rows, size_t cols, size_t ld, size_t size, bool written) {
-    add(p, name, rows && cols ? ((rows - 1) * ld + cols) * size : 0, size, written);
+  // rows x cols elements of `size` bytes, `ld` elements from row to row.  It may be the very array
+  // `same`, each row of which is read before it is written.
+  void matrix(const void *p, const char *name, size_t rows, size_t cols, size_t ld, size_t size, bool written,
+              const void *same = nullptr) {
+    add(p, name, rows && cols ? ((rows - 1) * ld + cols) * size : 0, size, written, same);
   }
-  // `bytes` bytes that begin at a multiple of `align`.
-  void add(const void *p, const char *name, size_t bytes, size_t align, bool written) {
-    if (p) spans_[count_++] = {static_cast<const char *>(p), bytes, align, name, written, nullptr};
-  }
-  // The operand added last may be the very array `p`: each row of `p` is read before it is written.
-  void or_same_as(const void *p) {
-    if (count_ && spans_[count_ - 1].p == p) spans_[count_ - 1].same = p;
+  // `bytes` bytes that begin at a multiple of `align`; nothing where `p` is NULL.
+  void add(const void *p, const char *name, size_t bytes, size_t align, bool written, const void *same = nullptr) {
+    if (p) spans_[count_++] = {static_cast<const char *>(p), bytes, align, name, written, same};
   }
 
   bool ok() const {
@@ -51,6 +49,11 @@ class Operands {
       if (check_symmetric(s.p, what.c_str()) && check_extent(s.p, s.bytes, what.c_str())) fail(what + " is not aligned to " + std::to_string(s.align) + " bytes");
       return false;
     }
+    return disjoint();
+  }
+
+  // No operand that is written shares bytes with another but the one that it may be.
+  bool disjoint() const {
     for (int i = 0; i < count_; ++i)
       for (int j = 0; j < i; ++j) {
         const Span &a = spans_[i], &b = spans_[j];

@@ -22,3 +22,26 @@ def test_rows_per_gate_means_nothing_without_a_gate(dtype, rows, cols, rows_per_
             c.fields["rows_per_gate"] = rows_per_gate
             run_forward(c)
             run_backward(c)
+
+
+def refused(call, args, word):
+    with pytest.raises(rs.RocShmemError, match=word):
+        call(args)
+
+
+@pytest.mark.parametrize("replicated", [False, True])
+def test_a_result_takes_no_other_results_place(replicated):
+    """Only `normed` may be `source` and only `grad_residual` may be `grad_residual_out`, also where a call
+    has neither: rows are read and written by workgroups of their own."""
+    with runtime(4):
+        c = NormCase(rs.FLOAT, 64, 512, 4, gate=0, pre_w=False, post=False, replicated=replicated)
+        source, x, out = c.rows_of(64, 512, 0), c.stream(), c.stream()
+        fields = dict(c.fields, source=source, residual=x)
+        refused(rs.roc_shmem_norm_to_all, rs.NormArgs(residual_out=source, **fields), "residual_out and source overlap")
+        rs.roc_shmem_norm_to_all(rs.NormArgs(residual_out=x, **fields))
+        grads = dict(c.fields, grad_residual_out=out)
+        wide = c.rows_of(64, 512, 0)
+        refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(grad_source=wide, **{**grads, "grad_residual_out": wide}),
+                "grad_source and grad_residual_out overlap")
+        rs.roc_shmem_norm_to_all_grad(rs.NormGradArgs(grad_source=wide, grad_residual=out, **grads))
+        rs.synchronize()
