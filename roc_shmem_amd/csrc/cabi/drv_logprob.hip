@@ -903,14 +903,14 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   if (a.rows == 0) return 0;
   const size_t size = type_size(a.dtype);
   rsm::Operands o(call);
-  o.matrix(a.logits, "logits", a.rows, width, s.ld, size, false);
+  const int logits = o.matrix(a.logits, "logits", a.rows, width, s.ld, size, false);
   o.add(a.tokens, "tokens", a.rows * 8, 8, false);
   o.add(a.lse, "lse", a.rows * 4, 4, false);
   o.add(a.entropy, "entropy", a.rows * 4, 4, false);
   o.add(a.grad_logprob, "grad_logprob", a.rows * 4, 4, false);
   o.add(a.grad_entropy, "grad_entropy", a.rows * 4, 4, false);
   o.add(a.grad_lse, "grad_lse", a.rows * 4, 4, false);
-  o.matrix(a.grad_logits, "grad_logits", a.rows, width, grad_ld, size, true, grad_ld == s.ld ? a.logits : nullptr);
+  o.matrix(a.grad_logits, "grad_logits", a.rows, width, grad_ld, size, true, grad_ld == s.ld ? logits : o.kNone);
   if (!o.ok()) return -1;
   LogprobBackward p{};
   p.rows = static_cast<int>(a.rows);

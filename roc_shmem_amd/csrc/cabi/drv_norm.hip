@@ -677,13 +677,13 @@ int rsm_norm_to_all(const rsm_norm_args_t *args, void *stream) {
   if (a.rows == 0) return 0;
   const size_t size = type_size(a.dtype), held = s.replicated ? a.rows : s.share, ld = static_cast<size_t>(s.residual_ld);
   rsm::Operands o(call);
-  o.matrix(a.source, "source", a.rows, a.cols, source_ld, size, false);
-  o.matrix(a.residual, "residual", held, a.cols, ld, size, false);
+  const int source = o.matrix(a.source, "source", a.rows, a.cols, source_ld, size, false);
+  const int residual = o.matrix(a.residual, "residual", held, a.cols, ld, size, false);
   o.add(a.pre_weight, "pre_weight", a.cols * size, size, false);
   o.add(a.post_weight, "post_weight", a.cols * size, size, false);
   o.add(a.gate, "gate", gate_rows(s) * a.cols * size, size, false);
-  o.matrix(a.residual_out, "residual_out", held, a.cols, ld, size, true, a.residual);
-  o.matrix(a.normed, "normed", a.rows, a.cols, normed_ld, size, true, normed_ld == source_ld ? a.source : nullptr);
+  o.matrix(a.residual_out, "residual_out", held, a.cols, ld, size, true, residual);
+  o.matrix(a.normed, "normed", a.rows, a.cols, normed_ld, size, true, normed_ld == source_ld ? source : o.kNone);
   o.matrix(a.total, "total", s.share, a.cols, a.cols, size, true);
   if (!o.ok()) return -1;
   NormForward p{};
@@ -735,15 +735,15 @@ int rsm_norm_to_all_grad(const rsm_norm_grad_args_t *args, void *stream) {
   const size_t size = type_size(a.dtype), held = s.replicated ? a.rows : s.share, ld = static_cast<size_t>(s.residual_ld);
   const size_t mine = a.rows ? held : 0, shared = a.rows ? s.share : 0;
   rsm::Operands o(call);
-  o.matrix(a.grad_normed, "grad_normed", a.rows, a.cols, normed_ld, size, false);
+  const int grad_normed = o.matrix(a.grad_normed, "grad_normed", a.rows, a.cols, normed_ld, size, false);
   o.matrix(a.residual_out, "residual_out", mine, a.cols, ld, size, false);
   o.matrix(a.total, "total", shared, a.cols, a.cols, size, false);
-  o.matrix(a.grad_residual_out, "grad_residual_out", mine, a.cols, ld, size, false);
+  const int grad_residual_out = o.matrix(a.grad_residual_out, "grad_residual_out", mine, a.cols, ld, size, false);
   o.add(a.pre_weight, "pre_weight", a.cols * size, size, false);
   o.add(a.post_weight, "post_weight", a.cols * size, size, false);
   o.add(a.gate, "gate", gate_rows(s) * a.cols * size, size, false);
-  o.matrix(a.grad_source, "grad_source", a.rows, a.cols, source_ld, size, true, source_ld == normed_ld ? a.grad_normed : nullptr);
-  o.matrix(a.grad_residual, "grad_residual", mine, a.cols, ld, size, true, a.grad_residual_out);
+  o.matrix(a.grad_source, "grad_source", a.rows, a.cols, source_ld, size, true, source_ld == normed_ld ? grad_normed : o.kNone);
+  o.matrix(a.grad_residual, "grad_residual", mine, a.cols, ld, size, true, grad_residual_out);
   o.add(a.grad_pre_weight, "grad_pre_weight", a.cols * 4, 4, true);
   o.add(a.grad_post_weight, "grad_post_weight", a.cols * 4, 4, true);
   o.add(a.grad_gate, "grad_gate", gate_rows(s) * a.cols * 4, 4, true);

@@ -25,15 +25,19 @@ class Operands {
  public:
   explicit Operands(const char *call) : call_(call) {}
 
-  // rows x cols elements of `size` bytes, `ld` elements from row to row.  It may be the very array
-  // `same`, each row of which is read before it is written.
-  void matrix(const void *p, const char *name, size_t rows, size_t cols, size_t ld, size_t size, bool written,
-              const void *same = nullptr) {
-    add(p, name, rows && cols ? ((rows - 1) * ld + cols) * size : 0, size, written, same);
+  static constexpr int kNone = -1;   // no operand
+
+  // rows x cols elements of `size` bytes, `ld` elements from row to row.  It may be the same array as the
+  // operand `may_be`, added before it, each row of which is read before it is written.  Returns the
+  // operand's number.
+  int matrix(const void *p, const char *name, size_t rows, size_t cols, size_t ld, size_t size, bool written, int may_be = kNone) {
+    return add(p, name, rows && cols ? ((rows - 1) * ld + cols) * size : 0, size, written, may_be);
   }
-  // `bytes` bytes that begin at a multiple of `align`; nothing where `p` is NULL.
-  void add(const void *p, const char *name, size_t bytes, size_t align, bool written, const void *same = nullptr) {
-    if (p) spans_[count_++] = {static_cast<const char *>(p), bytes, align, name, written, same};
+  // `bytes` bytes that begin at a multiple of `align`; no operand where `p` is NULL.
+  int add(const void *p, const char *name, size_t bytes, size_t align, bool written, int may_be = kNone) {
+    if (!p) return kNone;
+    spans_[count_] = {static_cast<const char *>(p), bytes, align, name, written, may_be};
+    return count_++;
   }
 
   bool ok() const {
@@ -52,13 +56,14 @@ class Operands {
     return disjoint();
   }
 
-  // No operand that is written shares bytes with another but the one that it may be.
+  // No operand that is written shares bytes with another but the one that it may be: with that operand, not
+  // with its array, which may serve as a further operand that is read in another order.
   bool disjoint() const {
     for (int i = 0; i < count_; ++i)
       for (int j = 0; j < i; ++j) {
         const Span &a = spans_[i], &b = spans_[j];
         if (!(a.written || b.written) || !(a.p < b.p + b.bytes && b.p < a.p + a.bytes)) continue;
-        if (a.p == b.p && ((a.same == b.p && !b.written) || (b.same == a.p && !a.written))) continue;
+        if (a.p == b.p && a.may_be == j) continue;
         fail(std::string(call_) + ": " + a.name + " and " + b.name + " overlap");
         return false;
       }
@@ -71,7 +76,7 @@ class Operands {
     size_t bytes, align;
     const char *name;
     bool written;
-    const void *same;
+    int may_be;
   };
   static constexpr int kMost = 16;   // no call has more operands
   const char *call_;

@@ -45,3 +45,23 @@ def test_a_result_takes_no_other_results_place(replicated):
                 "grad_source and grad_residual_out overlap")
         rs.roc_shmem_norm_to_all_grad(rs.NormGradArgs(grad_source=wide, grad_residual=out, **grads))
         rs.synchronize()
+
+
+@pytest.mark.parametrize("replicated", [False, True])
+def test_in_place_of_one_operand_is_not_in_place_of_two(replicated):
+    """One array may be read as two operands, and a result may replace either where nothing else reads its
+    array: the other operand's rows are read by other workgroups, at other places."""
+    with runtime(4):
+        c = NormCase(rs.FLOAT, 64, 512, 4, gate=0, pre_w=False, post=False, replicated=replicated)
+        both, out, h = c.rows_of(64, 512, 0), c.stream(), c.rows_of(64, 512, 0)
+        fields = dict(c.fields, source=both, residual=both)
+        refused(rs.roc_shmem_norm_to_all, rs.NormArgs(residual_out=both, normed=h, **fields), "residual_out and source overlap")
+        refused(rs.roc_shmem_norm_to_all, rs.NormArgs(residual_out=out, normed=both, **fields), "normed and residual overlap")
+        rs.roc_shmem_norm_to_all(rs.NormArgs(residual_out=out, normed=h, **fields))
+        grads = dict(c.fields, grad_normed=both, grad_residual_out=both, residual_out=out)
+        refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(grad_source=both, grad_residual=c.stream(), **grads),
+                "grad_source and grad_residual_out overlap")
+        refused(rs.roc_shmem_norm_to_all_grad, rs.NormGradArgs(grad_source=h, grad_residual=both, **grads),
+                "grad_residual and grad_normed overlap")
+        rs.roc_shmem_norm_to_all_grad(rs.NormGradArgs(grad_source=h, grad_residual=c.stream(), **grads))
+        rs.synchronize()
