@@ -80,7 +80,7 @@ __device__ __forceinline__ int column(int cols, int lane, int v) {
   return kEnd == kShifted && c < cols && c > cols - kRowVec<T> ? cols - kRowVec<T> : c;
 }
 // What a lane's element e of vector v counts in a sum over the row: its value, or 0 where the
-// neighbour counts it.
+// neighbour counts it.  Every factor that may be infinite goes through here: inf * 0 is NaN.
 template <typename T, int kLanes, int kEnd>
 __device__ __forceinline__ float counted(int cols, int lane, int v, int e, float value) {
   if constexpr (kEnd != kShifted) return value;
@@ -205,7 +205,10 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int e = 0; e < V; ++e) ss[0] = fmaf(acc[v][e], counted<T, kLanes, kEnd>(s.cols, lane, v, e, acc[v][e]), ss[0]);
+      for (int e = 0; e < V; ++e) {
+        const float sc = counted<T, kLanes, kEnd>(s.cols, lane, v, e, acc[v][e]);
+        ss[0] = fmaf(sc, sc, ss[0]);
+      }
     row_sums<kLanes>(ss, slots, turn);
     const float r = rsqrtf(fmaf(ss[0], s.inv_cols, s.eps));
 #pragma unroll
@@ -220,7 +223,8 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_kernel(NormForward p) {
     for (int e = 0; e < V; ++e) {
       const float z = acc[v][e] * row_get<T>(gate[v], e);
       acc[v][e] = fmaf(s.residual_scale, row_get<T>(x[v], e), s.block_scale * z);
-      ss[0] = fmaf(acc[v][e], counted<T, kLanes, kEnd>(s.cols, lane, v, e, acc[v][e]), ss[0]);
+      const float xc = counted<T, kLanes, kEnd>(s.cols, lane, v, e, acc[v][e]);
+      ss[0] = fmaf(xc, xc, ss[0]);
     }
   // The row may be stored over what a shifted lane of another wave still loads.
   if (kEnd == kShifted && kLanes > 64 && !s.post) __syncthreads();
@@ -325,11 +329,12 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float xe = row_get<T>(x[v], e), se = row_get<T>(tot[v], e);
-        const float xc = counted<T, kLanes, kEnd>(s.cols, lane, v, e, xe);
-        sums[0] = fmaf(xe, xc, sums[0]);
-        sums[1] = fmaf(d[v][e] * (s.pre_offset + row_get<T>(wpre[v], e)), xc, sums[1]);
-        sums[2] = fmaf(se, counted<T, kLanes, kEnd>(s.cols, lane, v, e, se), sums[2]);
+        const float xc = counted<T, kLanes, kEnd>(s.cols, lane, v, e, row_get<T>(x[v], e));
+        const float sc = counted<T, kLanes, kEnd>(s.cols, lane, v, e, row_get<T>(tot[v], e));
+        const float t = d[v][e] * (s.pre_offset + row_get<T>(wpre[v], e));
+        sums[0] = fmaf(xc, xc, sums[0]);
+        sums[1] = fmaf(counted<T, kLanes, kEnd>(s.cols, lane, v, e, t), xc, sums[1]);
+        sums[2] = fmaf(sc, sc, sums[2]);
       }
     row_sums<kLanes>(sums, slots, turn);
     keep_packed(x);
@@ -377,7 +382,7 @@ __global__ void __launch_bounds__(kWgLanes<kLanes>) norm_grad_kernel(NormBackwar
         f *= row_get<T>(g[v], e);
         to_post[e] = f * u;
         f *= w;
-        qs[0] = fmaf(counted<T, kLanes, kEnd>(s.cols, lane, v, e, f), u, qs[0]);
+        qs[0] = fmaf(counted<T, kLanes, kEnd>(s.cols, lane, v, e, f), counted<T, kLanes, kEnd>(s.cols, lane, v, e, u), qs[0]);
         d[v][e] = f;
       }
       if (p.part_post) add_to(sums_of[1], v, to_post);

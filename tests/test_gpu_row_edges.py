@@ -1,10 +1,12 @@
 """Row collectives at the edges of their contract."""
+import numpy as np
 import pytest
 
 import roc_shmem_amd as rs
+import row_reference as ref
 from helpers import runtime
+from test_gpu_norm_to_all import A, run_backward, run_forward
 from test_gpu_norm_to_all import Case as NormCase
-from test_gpu_norm_to_all import run_backward, run_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +67,71 @@ def test_in_place_of_one_operand_is_not_in_place_of_two(replicated):
                 "grad_residual and grad_normed overlap")
         rs.roc_shmem_norm_to_all_grad(rs.NormGradArgs(grad_source=h, grad_residual=c.stream(), **grads))
         rs.synchronize()
+
+
+# Columns of an infinity: the first, the last, and those that the last two vectors of a row both hold.
+ENDS = [(128, (0, 60, 127)), (131, (0, 125, 127, 128, 130)), (1030, (3, 1021, 1022, 1023, 1026, 1029)), (2051, (7, 2043, 2047, 2048, 2050))]
+
+
+@BOTH
+@pytest.mark.parametrize("cols,at", ENDS)
+def test_an_infinity_reaches_as_far_in_every_width(dtype, cols, at):
+    """A row with an infinite element has an infinite mean of squares, so r = 0: the rest of its normed row
+    is 0 and the element itself inf * 0.  The residual stream holds the infinity and its neighbours."""
+    with runtime(2):
+        c = NormCase(dtype, len(at), cols, 2, gate=0, post=False, replicated=True)
+        x, parts = c.numbers(len(at), cols), [c.numbers(len(at), cols) for _ in range(2)]
+        for row, col in enumerate(at):
+            x[row, col] = ref.to_type(dtype, [-np.inf if row % 2 else np.inf])[0]
+        source, h = c.rows_of(len(at), cols, 0).write_all(parts), c.rows_of(len(at), cols, 0)
+        out, res = c.stream(), c.stream(x)
+        rs.roc_shmem_norm_to_all(rs.NormArgs(source=source, residual=res, residual_out=out, normed=h, **c.fields))
+        rs.synchronize()
+        got, stream = ref.from_type(dtype, h.read(1)), ref.from_type(dtype, out.read(1))
+        hit = np.arange(cols)[None, :] == np.asarray(at)[:, None]
+        assert np.array_equal(np.isnan(got), hit)
+        assert not got[~hit].any()
+        assert np.array_equal(np.isinf(stream), hit) and not np.isnan(stream).any()
+
+
+@BOTH
+@pytest.mark.parametrize("cols,at", ENDS)
+def test_an_infinite_sum_reaches_as_far_in_every_width(dtype, cols, at):
+    """The same of the members' sum and the norm behind it: z = s r(s) is 0 but for inf * 0, so the residual
+    stream keeps its other elements."""
+    with runtime(2):
+        c = NormCase(dtype, len(at), cols, 2, gate=0, replicated=True)
+        x, parts = c.numbers(len(at), cols), [c.numbers(len(at), cols) for _ in range(2)]
+        for row, col in enumerate(at):
+            parts[1][row, col] = ref.to_type(dtype, [np.inf])[0]
+        source, out = c.rows_of(len(at), cols, 0).write_all(parts), c.stream()
+        fields = {k: v for k, v in c.fields.items() if k != "pre_weight"}
+        rs.roc_shmem_norm_to_all(rs.NormArgs(source=source, residual=c.stream(x), residual_out=out, **fields))
+        rs.synchronize()
+        got, hit = ref.from_type(dtype, out.read(0)), np.arange(cols)[None, :] == np.asarray(at)[:, None]
+        assert np.array_equal(np.isnan(got), hit)
+        want = A * ref.from_type(dtype, x)        # one product, exact, rounded once
+        assert (np.abs(got - want)[~hit] <= ref.HALF_STEP[dtype] * np.abs(want)[~hit]).all()
+
+
+@BOTH
+@pytest.mark.parametrize("cols,at", ENDS)
+def test_an_infinite_gradient_reaches_as_far_in_every_width(dtype, cols, at):
+    """mean(t n) is infinite where t is, so D = -n times it: infinite throughout, and NaN only at the element
+    itself where inf - inf meet."""
+    with runtime(2):
+        c = NormCase(dtype, len(at), cols, 2, gate=0, post=False, pre_w=False, replicated=True)
+        x = c.numbers(len(at), cols)
+        x[:] = ref.to_type(dtype, np.where(c.rng.random(x.shape) < 0.5, -1.0, 1.0) * (0.5 + c.rng.random(x.shape)))
+        parts = [c.numbers(len(at), cols) for _ in range(2)]
+        for row, col in enumerate(at):
+            parts[0][row, col] = ref.to_type(dtype, [np.inf])[0]
+        gn, gs, gr = c.rows_of(len(at), cols, 0).write_all(parts), c.rows_of(len(at), cols, 0), c.stream()
+        rs.roc_shmem_norm_to_all_grad(rs.NormGradArgs(grad_normed=gn, residual_out=c.stream(x), grad_source=gs, grad_residual=gr, **c.fields))
+        rs.synchronize()
+        hit = np.arange(cols)[None, :] == np.asarray(at)[:, None]
+        v = ref.from_type(dtype, x)
+        sign = -np.sign(v) * np.sign((v * hit).sum(1, keepdims=True))
+        for got in (ref.from_type(dtype, gs.read(1)), ref.from_type(dtype, gr.read(0))):
+            assert np.array_equal(np.isnan(got), hit)
+            assert np.array_equal(got[~hit], (sign * np.inf)[~hit])
