@@ -370,12 +370,13 @@ int rsm_norm_grad_work_bytes(const rsm_norm_grad_args_t *args, size_t *bytes);
  * m * shard .. min(vocab, (m + 1) * shard) - 1 (shard 0: ceil(vocab / team size)), one row per token
  * position.  With y = scale * logits over all members:
  *   lse = ln sum exp(y), logprob = y[token] - lse, entropy = -sum p ln p with p = exp(y - lse),
+ *   largest = max logits, log_sum = lse - scale * largest: the normaliser in two parts, exact where lse is not,
  * and the top_k largest logits (at most 32), equal ones by ascending id, with their log probabilities.
  * Results go to every member; those that are NULL are left out.  `tokens` (the first member's copy is
  * read) are ids; a negative one stands for a position without a token: logprob 0.  An id of vocab or
  * more gives NaN and raises the status word (rsm_take_status() == 2).  Logits at minus infinity are
- * outside the vocabulary; a row of nothing else has lse and log probabilities of minus infinity and
- * entropy 0.  A row with a NaN or plus infinity has NaN results; NaN logits are never alternatives, and
+ * outside the vocabulary; a row of nothing else has lse, both its parts and log probabilities of minus
+ * infinity and entropy 0.  A row with a NaN or plus infinity has NaN results; NaN logits are never alternatives, and
  * where fewer than top_k others are there the rest of the row is id -1 with NaN.
  * `work` (rsm_logprob_work_bytes() bytes, aligned to 16) and pSync (ROC_SHMEM_REDUCE_SYNC_SIZE longs, all
  * ROC_SHMEM_SYNC_VALUE on entry and on return) are symmetric arrays that no other call in flight uses;
@@ -394,14 +395,18 @@ typedef struct rsm_logprob_args {
   float *top_logprobs;                /* [rows][top_k] */
   void *work;
   long *pSync;
+  float *largest, *log_sum;           /* [rows] */
 } rsm_logprob_args_t;
 int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream);
 int rsm_logprob_work_bytes(const rsm_logprob_args_t *args, size_t *bytes);
 
 /* Its gradient: every member's part of the gradient of the logits, from the gradients of logprob,
  * entropy and lse (NULL: none; positions without a token have none of logprob) and what the forward
- * pass gave as lse and entropy (needed for grad_entropy).  The first member's copies of the arrays of
- * [rows] are read.  grad_logits may be `logits` (equal strides). */
+ * pass gave as lse - or, instead of it, as largest and log_sum - and entropy (needed for grad_entropy).  From
+ * lse a probability is off by lse's own rounding, up to 2^-24 |lse| of itself; largest and log_sum give the
+ * probabilities of the forward pass whatever the normaliser (a row that is all the type's lowest value has a lse of
+ * 1e38, in which ln vocab is lost).  The first member's copies of the arrays of [rows] are read.  grad_logits
+ * may be `logits` (equal strides). */
 typedef struct rsm_logprob_grad_args {
   int dtype;
   uint64_t team;
@@ -411,6 +416,7 @@ typedef struct rsm_logprob_grad_args {
   const int64_t *tokens;
   const float *lse, *entropy, *grad_logprob, *grad_entropy, *grad_lse;
   void *grad_logits;
+  const float *largest, *log_sum;     /* both, or neither and lse */
 } rsm_logprob_grad_args_t;
 int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream);
 

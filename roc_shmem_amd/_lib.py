@@ -56,12 +56,13 @@ NormGradArgs = _row_args(
 LogprobArgs = _row_args(
     "LogprobArgs", "rsm_logprob_args_t",
     [("dtype", i32), ("top_k", i32), ("team", u64), ("rows", sz), ("vocab", sz), ("shard", sz), ("logits_ld", sz),
-     ("scale", C.c_float)] + _pointers("logits tokens logprob entropy lse top_ids top_logprobs work pSync"), scale=1.0)
+     ("scale", C.c_float)] + _pointers("logits tokens logprob entropy lse top_ids top_logprobs work pSync largest log_sum"),
+    scale=1.0)
 LogprobGradArgs = _row_args(
     "LogprobGradArgs", "rsm_logprob_grad_args_t",
     [("dtype", i32), ("team", u64), ("rows", sz), ("vocab", sz), ("shard", sz), ("logits_ld", sz), ("grad_ld", sz),
      ("scale", C.c_float)] +
-    _pointers("logits tokens lse entropy grad_logprob grad_entropy grad_lse grad_logits"), scale=1.0)
+    _pointers("logits tokens lse entropy grad_logprob grad_entropy grad_lse grad_logits largest log_sum"), scale=1.0)
 
 # name -> (restype, argtypes); every symbol declared in include/rocshmem_mi355x.h
 SIGNATURES = {

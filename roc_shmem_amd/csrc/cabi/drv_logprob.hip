@@ -5,8 +5,10 @@
 //   l = sum exp(y - m)          lse = m + ln l
 //   logprob = y[token] - lse    entropy = ln l - sum exp(y - m) (y - m) / l
 //   top: the k largest x, equal ones by ascending id, with their log probabilities
-// and backwards, with p = exp(y - lse):
-//   dx = c (g_logprob (1[token] - p) + g_lse p - g_entropy p (y - lse + entropy))
+// and backwards, with p = exp(y - lse) = exp(c (x - max x) - ln l):
+//   dx = c (g_logprob (1[token] - p) + g_lse p - g_entropy p (ln p + entropy))
+// The second form of p is the forward pass's own, good whatever the size of lse; the first, from lse as a
+// float, has p off by 2^-24 |lse| of itself.
 //
 // The forward pass reads every logit once.  A lane keeps a running maximum m of its own x, and
 // l = sum 2^((x - m) c2) and w = sum 2^((x - m) c2) (x - m) c2, c2 = c log2(e), against it; when m
@@ -41,7 +43,7 @@ struct LogprobForward {
   float scale;
   const char *logits;
   const int64_t *tokens;
-  char *logprob, *entropy, *lse, *top_ids, *top_logprobs;
+  char *logprob, *entropy, *lse, *largest, *log_sum, *top_ids, *top_logprobs;
   // A row is cut into batches of kBatch elements, 64 lanes x kDeep vectors, in ascending order of ids;
   // workgroup q of `parts` takes its share of them in order.  Either every member's part is cut for
   // itself (batches_per_member), or, where that would leave the last batches mostly empty (kPacked),
@@ -334,6 +336,8 @@ __device__ __forceinline__ void finish_row(const LogprobForward &p, int row, Sof
     if (p.logprob) reinterpret_cast<float *>(p.logprob + m * p.step)[row] = logprob;
     if (p.entropy) reinterpret_cast<float *>(p.entropy + m * p.step)[row] = entropy;
     if (p.lse) reinterpret_cast<float *>(p.lse + m * p.step)[row] = lse;
+    if (p.largest) reinterpret_cast<float *>(p.largest + m * p.step)[row] = empty ? -INFINITY : a.m;
+    if (p.log_sum) reinterpret_cast<float *>(p.log_sum + m * p.step)[row] = empty ? -INFINITY : log_l;
   }
   if constexpr (kTop) {
     if (lane < p.top_k) {
@@ -561,7 +565,8 @@ struct LogprobBackward {
   float scale;
   const char *logits;
   const int64_t *tokens;
-  const float *lse, *entropy, *grad_logprob, *grad_entropy, *grad_lse;
+  const float *largest, *normaliser;   // of a row: ln p = scale (x - largest) - normaliser; largest null: 0
+  const float *entropy, *grad_logprob, *grad_entropy, *grad_lse;
   char *grad_logits;
   // A line is one member's part of a row.  Either `chunks` workgroups take a line, or, where that would
   // leave them mostly idle (kPacked), the lines' vectors (vecs of them to a line) are numbered through.
@@ -578,15 +583,19 @@ constexpr int kGradChunk = kGradLanes * kRowVec<T> * kGradDeep;
 
 // What the gradient of a row's logits depends on.
 struct RowGrads {
-  float lse, of_token, of_entropy, flat;
+  float largest, normaliser, of_token, of_entropy, flat;
   int64_t token;
 };
 __device__ __forceinline__ RowGrads row_grads(const LogprobBackward &p, int row) {
   RowGrads r;
-  // A row without any logit above minus infinity has no probabilities: 0 throughout, as against an
-  // infinite normaliser.
-  r.lse = p.lse[row];
-  if (r.lse == -INFINITY) r.lse = INFINITY;
+  r.largest = p.largest ? p.largest[row] : 0.f;
+  r.normaliser = p.normaliser[row];
+  // A row without any logit above minus infinity has no probabilities: they are 0 throughout, as against
+  // an infinite normaliser, and what is left of its gradient is the token's own term.
+  if (r.normaliser == -INFINITY) {
+    r.largest = 0.f;
+    r.normaliser = INFINITY;
+  }
   r.token = p.tokens ? p.tokens[row] : -1;
   r.of_token = p.grad_logprob && r.token >= 0 && r.token < p.vocab ? p.scale * p.grad_logprob[row] : 0.f;
   r.of_entropy = p.grad_entropy ? p.scale * p.grad_entropy[row] : 0.f;
@@ -601,7 +610,7 @@ __device__ __forceinline__ u32x4 grad_of(const LogprobBackward &p, const RowGrad
   float d[kRowVec<T>];
 #pragma unroll
   for (int e = 0; e < kRowVec<T>; ++e) {
-    const float lp = fmaf(row_get<T>(raw, e), p.scale, -r.lse);
+    const float lp = fmaf(row_get<T>(raw, e) - r.largest, p.scale, -r.normaliser);
     d[e] = exp2_of(lp * kLog2e) * fmaf(-r.of_entropy, fmaxf(lp, kFarBelow), r.flat);
     if (e == hit) d[e] += r.of_token;
   }
@@ -828,7 +837,7 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
   LogprobShape s;
   if (!a.logits) return rsm::fail("logprob_to_all: logits must be given");
   if (a.logprob && !a.tokens) return rsm::fail("logprob_to_all: logprob without tokens");
-  if (!a.logprob && !a.entropy && !a.lse && !a.top_ids && !a.top_logprobs) return rsm::fail("logprob_to_all: no result is asked for");
+  if (!a.logprob && !a.entropy && !a.lse && !a.largest && !a.log_sum && !a.top_ids && !a.top_logprobs) return rsm::fail("logprob_to_all: no result is asked for");
   if ((a.top_ids || a.top_logprobs) != (a.top_k > 0)) return rsm::fail("logprob_to_all: top_k and the arrays for the alternatives do not go together");
   if (!top_in_range(call, a.top_k, a.vocab) || !shape_of(a, call, &s)) return -1;
   const LogprobPlan g = plan_of(s, a.dtype, a.rows, a.vocab, a.top_k);
@@ -841,6 +850,8 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
   o.add(a.logprob, "logprob", a.rows * 4, 4, true);
   o.add(a.entropy, "entropy", a.rows * 4, 4, true);
   o.add(a.lse, "lse", a.rows * 4, 4, true);
+  o.add(a.largest, "largest", a.rows * 4, 4, true);
+  o.add(a.log_sum, "log_sum", a.rows * 4, 4, true);
   o.add(a.top_ids, "top_ids", a.rows * a.top_k * 4, 4, true);
   o.add(a.top_logprobs, "top_logprobs", a.rows * a.top_k * 4, 4, true);
   if (g.parts > 1) {
@@ -862,6 +873,8 @@ int rsm_logprob_to_all(const rsm_logprob_args_t *args, void *stream) {
   p.logprob = moved(a.logprob, s.team.first);
   p.entropy = moved(a.entropy, s.team.first);
   p.lse = moved(a.lse, s.team.first);
+  p.largest = moved(a.largest, s.team.first);
+  p.log_sum = moved(a.log_sum, s.team.first);
   p.top_ids = moved(a.top_ids, s.team.first);
   p.top_logprobs = moved(a.top_logprobs, s.team.first);
   p.batches = g.batches;
@@ -892,7 +905,9 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   if (!args) return rsm::fail("logprob_to_all_grad: arguments are NULL");
   const rsm_logprob_grad_args_t &a = *args;
   LogprobShape s;
-  if (!a.logits || !a.lse || !a.grad_logits) return rsm::fail("logprob_to_all_grad: logits, lse and grad_logits must be given");
+  if (!a.largest != !a.log_sum) return rsm::fail("logprob_to_all_grad: largest and log_sum go together");
+  if (!a.logits || !a.grad_logits || !(a.lse || a.log_sum))
+    return rsm::fail("logprob_to_all_grad: logits, grad_logits and lse (or largest and log_sum) must be given");
   if (!a.grad_logprob && !a.grad_entropy && !a.grad_lse) return rsm::fail("logprob_to_all_grad: no gradient is given");
   if (a.grad_logprob && !a.tokens) return rsm::fail("logprob_to_all_grad: grad_logprob without tokens");
   if (a.grad_entropy && !a.entropy) return rsm::fail("logprob_to_all_grad: grad_entropy without entropy");
@@ -906,6 +921,8 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   const int logits = o.matrix(a.logits, "logits", a.rows, width, s.ld, size, false);
   o.add(a.tokens, "tokens", a.rows * 8, 8, false);
   o.add(a.lse, "lse", a.rows * 4, 4, false);
+  o.add(a.largest, "largest", a.rows * 4, 4, false);
+  o.add(a.log_sum, "log_sum", a.rows * 4, 4, false);
   o.add(a.entropy, "entropy", a.rows * 4, 4, false);
   o.add(a.grad_logprob, "grad_logprob", a.rows * 4, 4, false);
   o.add(a.grad_entropy, "grad_entropy", a.rows * 4, 4, false);
@@ -923,7 +940,8 @@ int rsm_logprob_to_all_grad(const rsm_logprob_grad_args_t *args, void *stream) {
   p.scale = a.scale;
   p.logits = moved(a.logits, s.team.first);
   p.tokens = moved_as<int64_t>(a.tokens, s.team.first);
-  p.lse = moved_as<float>(a.lse, s.team.first);
+  p.largest = moved_as<float>(a.largest, s.team.first);
+  p.normaliser = moved_as<float>(a.log_sum ? a.log_sum : a.lse, s.team.first);
   p.entropy = moved_as<float>(a.entropy, s.team.first);
   p.grad_logprob = moved_as<float>(a.grad_logprob, s.team.first);
   p.grad_entropy = moved_as<float>(a.grad_entropy, s.team.first);

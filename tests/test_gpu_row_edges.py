@@ -5,6 +5,9 @@ import pytest
 import roc_shmem_amd as rs
 import row_reference as ref
 from helpers import runtime
+from row_arrays import Rows
+from test_gpu_logprob_to_all import NP
+from test_gpu_logprob_to_all import Case as LogprobCase
 from test_gpu_norm_to_all import A, run_backward, run_forward
 from test_gpu_norm_to_all import Case as NormCase
 
@@ -135,3 +138,74 @@ def test_an_infinite_gradient_reaches_as_far_in_every_width(dtype, cols, at):
         for got in (ref.from_type(dtype, gs.read(1)), ref.from_type(dtype, gr.read(0))):
             assert np.array_equal(np.isnan(got), hit)
             assert np.array_equal(got[~hit], (sign * np.inf)[~hit])
+
+
+def rows_of_large_normalisers(rng, dtype, rows, vocab):
+    """Logits of 64 bits, rounded to the type, whose normalisers lose digits or all of them as floats."""
+    lowest = -3.3895314e38
+    base = rng.standard_normal((rows, vocab)) * 2
+    kinds = [np.full((rows, vocab), lowest), np.where(np.arange(vocab) % 7 == 3, lowest / 2, lowest), np.full((rows, vocab), -lowest),
+             np.where(rng.random((rows, vocab)) < 0.5, lowest, base), base - 3000, np.full((rows, vocab), -np.inf), base,
+             np.round(base) + 1e6 if dtype == rs.FLOAT else np.round(base) * 32 + 4096]
+    logits = np.empty((rows, vocab))
+    for row in range(rows):
+        logits[row] = kinds[row % len(kinds)][row]
+    return ref.to_type(dtype, logits)
+
+
+@BOTH
+@pytest.mark.parametrize("rows,vocab,scale", [(8, 3000, 1.0), (8, 40000, 1.0), (9, 40000, 2.5), (300, 3000, 0.75), (264, 9001, 1.0)])
+def test_gradients_where_the_normaliser_is_large(dtype, rows, vocab, scale):
+    """From largest and log_sum the gradient has the forward pass's probabilities, also in rows that are all
+    the type's lowest or highest value, or whose scaled normaliser is no float at all."""
+    rng = np.random.default_rng(rows + vocab)
+    with runtime(3, heap_size=256 << 20):
+        c = LogprobCase(dtype, rows, vocab, 3, logits=ref.from_type(dtype, rows_of_large_normalisers(rng, dtype, rows, vocab)),
+                        scale=scale, tokens=rng.integers(-1, vocab, rows))
+        out = {n: Rows(1, rows, np.float32) for n in ("logprob", "entropy", "largest", "log_sum")}
+        for a in out.values():
+            a.remember()
+        rs.roc_shmem_logprob_to_all(c.call(out))
+        rs.synchronize()
+        got = {n: a.read(2)[0] for n, a in out.items()}
+        for n, a in out.items():
+            for pe in range(3):
+                assert np.array_equal(a.read(pe)[0], got[n], equal_nan=True)
+                a.check_rest(pe, n, 1)
+        x = c.f64()
+        m = x.max(1)
+        empty = m == -np.inf
+        assert np.array_equal(got["largest"], m.astype(np.float32))
+        # the formulas on logits whose largest is 0: the same rows with a normaliser of ln l
+        below = x - np.where(empty, 0, m)[:, None]
+        want = ref.logprob_forward(below, c.tokens, c.scale, 0)
+        for n, of in (("log_sum", "lse"), ("entropy", "entropy"), ("logprob", "logprob")):
+            ref.check(n, rs.FLOAT, got[n], *want[of])
+        g = {n: rng.standard_normal(rows).astype(np.float32) for n in ("grad_logprob", "grad_entropy", "grad_lse")}
+        value, error = ref.logprob_backward(below, c.tokens, got["log_sum"], got["entropy"], c.scale, *g.values())
+        for in_place in (False, True):
+            d = c.array if in_place else Rows(rows, c.width, NP[dtype], c.ld)
+            fields = dict(entropy=out["entropy"], largest=out["largest"], log_sum=out["log_sum"], grad_logits=d, grad_ld=d.ld)
+            rs.roc_shmem_logprob_to_all_grad(rs.LogprobGradArgs(**fields, **{n: c.numbers(v, np.float32) for n, v in g.items()}, **c.fields))
+            rs.synchronize()
+            for pe in range(3):
+                part = slice(pe * c.shard, min(vocab, (pe + 1) * c.shard))
+                ref.check("grad_logits on PE %d" % pe, dtype, d.read(pe)[:, :part.stop - part.start], value[:, part], error[:, part])
+
+
+def test_largest_and_log_sum_alone_and_where_rows_are_not_numbers():
+    logits = np.random.default_rng(3).standard_normal((4, 5000)).astype(np.float32)
+    logits[1, 77], logits[2, 4999] = np.nan, np.inf
+    with runtime(2):
+        c = LogprobCase(rs.FLOAT, 4, 5000, 2, logits=logits)
+        m, s = Rows(1, 4, np.float32), Rows(1, 4, np.float32)
+        rs.roc_shmem_logprob_to_all(c.call({"largest": m}))
+        rs.roc_shmem_logprob_to_all(c.call({"log_sum": s}))
+        d = Rows(4, c.width, np.float32, c.ld)
+        rs.roc_shmem_logprob_to_all_grad(rs.LogprobGradArgs(largest=m, log_sum=s, grad_lse=c.numbers(np.ones(4), np.float32), grad_logits=d,
+                                                            **c.fields))
+        rs.synchronize()
+        assert np.array_equal(np.isnan(s.read(1)[0]), [False, True, True, False])
+        assert np.array_equal(m.read(1)[0][[0, 3]], logits[[0, 3]].max(1))
+        got = d.read(0)
+        assert np.isnan(got[1:3]).all() and np.isfinite(got[[0, 3]]).all()

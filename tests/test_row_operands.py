@@ -1,8 +1,10 @@
-"""The row collectives' check of operands against each other, on addresses alone."""
+"""What the row collectives refuse of operands that do not go together, without a GPU."""
 import os
 import subprocess
 
 import pytest
+
+import roc_shmem_amd as rs
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HIPCC = "/opt/rocm/bin/hipcc"
@@ -19,3 +21,12 @@ def test_operands_may_be_one_array_only_where_the_call_says_so(tmp_path):
     assert made.returncode == 0, made.stderr
     ran = subprocess.run([program], capture_output=True, text=True, timeout=60)
     assert ran.stdout == "ok\n" and ran.returncode == 0, ran.stdout + ran.stderr
+
+
+def test_the_parts_of_a_normaliser_go_together():
+    good = dict(dtype=rs.FLOAT, team=1, rows=4, vocab=8, logits=128, grad_lse=128, grad_logits=128)
+    for change, word in [(dict(), "lse"), (dict(largest=128), "largest"), (dict(log_sum=128), "largest"), (dict(lse=128, log_sum=128), "largest"),
+                         (dict(lse=128, largest=128), "log_sum"), (dict(lse=128), "rsm_init"), (dict(largest=128, log_sum=128), "rsm_init"),
+                         (dict(lse=128, largest=128, log_sum=128), "rsm_init")]:
+        with pytest.raises(rs.RocShmemError, match=word):
+            rs.roc_shmem_logprob_to_all_grad(rs.LogprobGradArgs(**good, **change))
