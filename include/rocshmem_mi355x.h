@@ -306,8 +306,8 @@ int rsm_barrier_all(int iterations, const rsm_launch_t *launch);
  * `dtype` says; sums and everything between are 32-bit floats, every result is rounded once, and
  * every run gives the same bits.  Row strides (*_ld) are in elements, 0 = packed rows; rows may
  * start at any element.  A call checks its operands as the other entry points do, refuses results
- * that overlap other operands (one array for both is allowed where it says so), and writes nothing
- * beyond the rows and columns it names. */
+ * that overlap other operands (one array for both is allowed where it says so, unless a third operand is
+ * that array too), and writes nothing beyond the rows and columns it names. */
 
 enum rsm_norm_flags {
   RSM_NORM_POST = 1,        /* the members' sum goes through a norm of its own               */
@@ -326,7 +326,8 @@ enum rsm_norm_flags {
  * owners.  The weights (cols elements) and `gate` (one packed row for every rows_per_gate rows of the
  * batch; 0 = one row for all; without a gate the field is not looked at) hold the same values on every
  * member.  `normed` may be NULL, may be `source` (equal strides), and residual_out may be `residual`.
- * cols <= 16384, rows < 2^22, eps a positive normal float.  Means of squares are 32-bit floats: a row whose mean square overflows comes out as zeros. */
+ * cols <= 16384, rows < 2^22, eps a positive normal float.  Squares are summed in 32-bit floats: a row whose
+ * sum of squares overflows comes out of its norm as zeros, and as NaN where an element is infinite. */
 typedef struct rsm_norm_args {
   int dtype;
   int flags;                 /* rsm_norm_flags */
@@ -377,7 +378,8 @@ int rsm_norm_grad_work_bytes(const rsm_norm_grad_args_t *args, size_t *bytes);
  * more gives NaN and raises the status word (rsm_take_status() == 2).  Logits at minus infinity are
  * outside the vocabulary; a row of nothing else has lse, both its parts and log probabilities of minus
  * infinity and entropy 0.  A row with a NaN or plus infinity has NaN results; NaN logits are never alternatives, and
- * where fewer than top_k others are there the rest of the row is id -1 with NaN.
+ * where fewer than top_k others are there the rest of the row is id -1 with NaN.  Differences of logits are
+ * 32-bit floats: one further below the largest than a float can tell counts as minus infinity.
  * `work` (rsm_logprob_work_bytes() bytes, aligned to 16) and pSync (ROC_SHMEM_REDUCE_SYNC_SIZE longs, all
  * ROC_SHMEM_SYNC_VALUE on entry and on return) are symmetric arrays that no other call in flight uses;
  * the first member's copies serve batches of fewer than 256 rows, and larger ones need neither (0

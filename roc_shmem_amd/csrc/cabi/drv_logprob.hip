@@ -758,7 +758,8 @@ LogprobPlan plan_of(const LogprobShape &s, int dtype, size_t rows, size_t vocab,
   // Many rows that are not long: half as many waves to a row and twice as many rows at a time, since a row's
   // waves stand idle while one of them ranks and joins (8 alternatives, 8 and 4 waves: 8192 x 20000 bf16 over 2
   // members 99.9 and 80.7 us, 8192 x 16000 74.0 and 68.3, 4096 x 50257 over 4 103 and 98; 4096 x 131072 over 8,
-  // 64 batches, 186 and 187; without alternatives 2048 x 32000 27.2 and 28.7, 8192 x 20000 72.8 and 67.6).
+  // 64 batches, 186 and 187.  Without alternatives nobody ranks and the rule is worth little: 2048 x 32000 loses,
+  // 27.2 and 28.7, 8192 x 20000 gains, 72.8 and 67.6.)
   const int most_waves = rows >= 2048 && all <= 32 ? kMaxWaves / 2 : kMaxWaves;
   g.waves = mine < most_waves ? static_cast<int>(mine) : most_waves;
   if (g.parts > 1) g.work_bytes = rows * g.parts * (sizeof(float4) + static_cast<size_t>(top_k) * 8);

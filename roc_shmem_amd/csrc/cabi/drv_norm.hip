@@ -633,9 +633,10 @@ GradPlan plan_of(const NormShape &s, int dtype, bool has_gate) {
   g.lanes = lanes_for(s.cols, dtype == RSM_BF16 ? 8 : 4, true);
   // Enough units to fill the chip's 256 compute units, no more: each leaves its sums behind.  (Rows of a
   // wave, 8192 x 64 bf16 over 8 members: 1024 units 26.6 us, 2048 21.2, 4096 21.8.  Rows of 256 lanes, 512
-  // units and 1024: 8192 x 2048 bf16 over 8 members 127 and 137, over 4 83 and 91, 8192 x 1200 over 3 62 and 52,
-  // whose fewer loads leave a unit's lanes waiting.  Rows of 512 lanes, 512 units and 1024: 8192 x 4096 over 4
-  // members 162 and 167, over 1 98 and 109.)
+  // units and 1024: 8192 x 2048 bf16 over 8 members 127 and 137, over 4 83 and 91, 8192 x 1200 over 3 62 and 52:
+  // width and members change together there, and the rule puts it down to the members, whose fewer loads leave
+  // a unit's lanes waiting; 106 of 256 lanes without an element may do it as well.  Rows of 512 lanes, 512
+  // units and 1024: 8192 x 4096 over 4 members 162 and 167, over 1 98 and 109.)
   const int64_t target = g.lanes.lanes == 64 ? 2048 : g.lanes.lanes == 256 && s.members < 4 ? 1024 : g.lanes.lanes == 1024 ? 256 : 512;
   const int64_t per_unit = (s.rows + target - 1) / target;
   const int64_t group = s.rows_per_gate;
